@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define FP4X_ABI_VERSION 13
+#define FP4X_ABI_VERSION 14
 
 enum {
   FP4X_OK = 0,
@@ -60,6 +60,7 @@ enum {
 
 /* weight-preparation sources and targets (fp4x_quantize, fp4x_absmax) */
 enum { FP4X_SRC_F32 = 0, FP4X_SRC_BF16 = 1, FP4X_SRC_MX8 = 2, FP4X_SRC_NV4 = 3 };
+enum { FP4X_Q8_INT8 = 0, FP4X_Q8_E4M3 = 1, FP4X_Q8_MX8 = 2 };  /* rows in 8 bits (fp4x_*_q8) */
 enum { FP4X_Q_W8 = 0, FP4X_Q_W6 = 1, FP4X_Q_NV4 = 2, FP4X_Q_INT2 = 3, FP4X_Q_INT2_E4M3 = 4 };
 
 const char* fp4x_last_error(void);
@@ -252,6 +253,43 @@ int fp4x_absmax(int src, const void* src_a, const void* src_b, float src_gs, int
  * [quantize_nv4, x/fp4x_kernels.py:277-300] */
 int fp4x_quantize_nv4(int src, const void* src_a, const void* src_b, float src_gs, int64_t N, int K, float* amax,
                       void* P, void* S, void* stream);
+
+/* Rows in 8 bits with scales, one launch.  A row v of H fp32 values ends as
+ *   FP4X_Q8_INT8  int8 rint(v / s), s fp32 [M] = max(amax, 1e-12) / 127
+ *   FP4X_Q8_E4M3  e4m3fn(v / s),    s fp32 [M] = max(amax, 1e-12) / 448
+ *   FP4X_Q8_MX8   MXFP8: e4m3fn(v / 2^X) saturating at 448, s e8m0 [M, H/32]
+ *                 = X + 127, X = floor(log2 amax) - 8 per 32 values; H % 32 == 0
+ * (IEEE fp32 division, round half to even).  A row (MXFP8: a block) with an
+ * infinity or a NaN gets the scale NaN (255) and codes 0 (NaN codes).  H is
+ * 1 .. 32768.  Rows are bf16, fp16 or fp32 (dtype) with unit column stride and
+ * any row stride (elements); every tensor needs its element's alignment only.
+ * q has row stride q_stride bytes >= H.  No counterpart in the reference (its
+ * host framework's norms and quantizers feed the products it replaces).
+ *
+ * rms_norm_q8: h = x + res rounded to res_dtype (x itself when res is NULL);
+ * v = (h * rs) * (w + w_offset), rs = fp32(1 / sqrt(mean(h^2) + eps)), the mean
+ * in fp64.  res and w have x's dtype or are fp32.  res_out (optional, res_dtype)
+ * receives h and may be res itself; normed (optional, dtype) receives v. */
+int fp4x_rms_norm_q8(const void* x, int64_t x_stride, int dtype, const void* res, int64_t res_stride, int res_dtype,
+                     const void* w, int w_dtype, float w_offset, double eps, int M, int H, int fmt, void* q,
+                     int64_t q_stride, void* s, void* res_out, int64_t res_out_stride, void* normed,
+                     int64_t normed_stride, void* stream);
+/* v = silu(gate) * up, within a few fp32 ulps before the quantization. */
+int fp4x_silu_mul_q8(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int dtype, int M, int F,
+                     int fmt, void* q, int64_t q_stride, void* s, void* stream);
+/* v = x (activations per token, or a weight per output channel). */
+int fp4x_quantize_q8(const void* x, int64_t x_stride, int dtype, int M, int H, int fmt, void* q, int64_t q_stride,
+                     void* s, void* stream);
+
+/* out[m, n] = cast(((sum_k xq[m, k] * wq[n, k]) * xs[m]) * ws[n] + bias[n]):
+ * int8 codes, the sum exact in int32 (K <= 131071), then rounded fp32 steps, so
+ * results do not depend on the launch shape.  xs fp32 [M], ws and bias (NULL:
+ * none) fp32 [N].  Code rows start on 16 bytes (strides a multiple of 16) and
+ * are readable to the next 16-byte boundary past K; what is there is ignored.
+ * Any M, N and K.  No counterpart in the reference. */
+int fp4x_w8a8_linear(const void* xq, int64_t x_stride, const float* xs, const void* wq, int64_t w_stride,
+                     const float* ws, const float* bias, void* out, int64_t out_stride, int out_dtype, int M, int N,
+                     int K, void* stream);
 
 /* Mixer down projection: split-K W8 GEMV whose last workgroup per row tile
  * writes di = bf16(sum) [M, N] and bot = bf16(sc * sigmoid(sc)) [M, lr] with

@@ -44,6 +44,11 @@ _SIGS = {
     "fp4x_quantize_w6_clip": ([_I, _P, _P, ctypes.c_float, _I64, _I, _I, _I, _P, _P, _P, _P], _I),
     "fp4x_quantize_nv4": ([_I, _P, _P, ctypes.c_float, _I64, _I, _P, _P, _P, _P], _I),
     "fp4x_absmax": ([_I, _P, _P, ctypes.c_float, _I64, _I, _P, _P], _I),
+    "fp4x_rms_norm_q8": ([_P, _I64, _I, _P, _I64, _I, _P, _I, _F, ctypes.c_double, _I, _I, _I, _P, _I64, _P, _P, _I64,
+                          _P, _I64, _P], _I),
+    "fp4x_silu_mul_q8": ([_P, _I64, _P, _I64, _I, _I, _I, _I, _P, _I64, _P, _P], _I),
+    "fp4x_quantize_q8": ([_P, _I64, _I, _I, _I, _I, _P, _I64, _P, _P], _I),
+    "fp4x_w8a8_linear": ([_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _P], _I),
     "fp4x_hc_down": ([_P, _I64, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P], _I),
     "fp4x_hc_up": ([_P, _I64, _P, _P, _I, _P, _I64, _P, _I, _I, _I, _I, _I, _P], _I),
     "fp4x_hc_mix": ([_P, _I64, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _P, _I64, _P, _I, _I,
@@ -56,7 +61,7 @@ _SIGS = {
     "fp4x_read_ceiling": ([_P, _I64, _I, _I, _P, _P], _I),
     "fp4x_hold_cus": ([_I, _I64, _I, _P, _P], _I),
 }
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _LIB = None
 

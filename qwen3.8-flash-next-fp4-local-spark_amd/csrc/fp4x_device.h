@@ -94,6 +94,20 @@ __device__ __forceinline__ float ubyte_to_f32(uint32_t v) {
   return (float)((v >> (8 * B)) & 0xffu);
 }
 
+// ---------------------------------------------------------------- quantizers
+constexpr float kRint = 12582912.0f;               // 1.5 * 2^23: v + kRint holds rint(v) in its low bits
+
+// RN(f / s) from rs = RN(1 / s) (Markstein: a quotient within an ulp, its exact
+// remainder by fma, and one correction with the rounded reciprocal give the
+// rounded quotient), for 2^-100 <= s < 2^100 and finite f; a quotient so small
+// that the remainder underflows is still within an ulp, which no code notices.
+// -0 gives +0.
+__device__ __forceinline__ float exact_quot(float f, float s, float rs) {
+  const float q = f * rs;
+  return __builtin_fmaf(__builtin_fmaf(-q, s, f), rs, q);
+}
+__device__ __forceinline__ bool mid_range(float s) { return s >= 0x1p-100f && s < 0x1p100f; }
+
 // ---------------------------------------------------------------- lanes
 // Butterfly all-reduce over groups of `n` consecutive lanes (n a power of
 // two <= 64): step s = 1, 2, 4, ... adds the partner lane (lane ^ s).  Each

@@ -180,19 +180,6 @@ __device__ __forceinline__ bool finite_max(float m) { return m < __builtin_inff(
 
 // Targets: put(t, f) quantizes weights [16 t, 16 t + 16) of the matrix; lanes
 // t of one group run together.
-constexpr float kRint = 12582912.0f;               // 1.5 * 2^23: v + kRint holds rint(v) in its low bits
-
-// RN(f / s) from rs = RN(1 / s) (Markstein: a quotient within an ulp, its exact
-// remainder by fma, and one correction with the rounded reciprocal give the
-// rounded quotient), for 2^-100 <= s < 2^100 and finite f; a quotient so small
-// that the remainder underflows is still within an ulp, which no code notices.
-// -0 gives +0.
-__device__ __forceinline__ float exact_quot(float f, float s, float rs) {
-  const float q = f * rs;
-  return __builtin_fmaf(__builtin_fmaf(-q, s, f), rs, q);
-}
-__device__ __forceinline__ bool mid_range(float s) { return s >= 0x1p-100f && s < 0x1p100f; }
-
 // ------------------------------------------------------------------ targets
 // W8 g64: s = max(amax, 1e-12) / 127, q = clamp(rint(w / s), -127, 127).
 // The clamp never acts on a finite group: its maximum gives 127.

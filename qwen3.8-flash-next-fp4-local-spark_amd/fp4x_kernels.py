@@ -25,6 +25,7 @@ import _fp4x as _L
 __all__ = [
     "mx8_linear", "bf16_linear", "nv4_linear", "w8_linear", "w6_linear", "int2_logits", "refine_mx8_", "refine_nv4",
     "scatter_draft", "draft_nv4",
+    "rms_norm_q8", "silu_mul_q8", "quantize_q8", "w8a8_linear",
     "topk_rows", "int2_topk", "w8_linear_layers", "HCFused", "hc_scaled_silu", "hc_gate_mean",
     "quantize_w8", "quantize_w6", "quantize_nv4", "quantize_int2", "quantize_mx8",
     "mx8_dequant", "dequant_int2", "dequant_nv4", "dequant_operand", "requantize_mx8", "requantize_nv4", "ORDER",
@@ -195,6 +196,186 @@ def nv4_linear(x2, wp, s, gs, cfg=(32, 256, 4), out_dtype=torch.bfloat16):
     ks = _check_split(k, cfg, ks_idx=3)
     return _linear(_L.lib().fp4x_nv4_linear, _L.FMT_NV4, x2, n, k, ks, out_dtype, (_ptr(wp), _ptr(s), float(gs)),
                    (_ptr(wp), None, _ptr(s)), float(gs))
+
+
+# ----------------------------------------------------------------- 8-bit activations
+# fmt -> (the library's code, the codes' dtype)
+_Q8 = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn), "mx8": (2, torch.float8_e4m3fn)}
+
+
+def _same_gpu(x, *ts):
+    d = x.get_device()
+    if d < 0:
+        raise RuntimeError("fp4x: HIP kernels need GPU tensors")
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise RuntimeError("fp4x: HIP kernels need GPU tensors, all on one GPU")
+
+
+def _rows2(t, what):
+    """2-D rows with unit column stride (copied where they have another)."""
+    if t.dim() != 2:
+        raise ValueError(f"fp4x: {what} must be 2-D")
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _q8_out(x, m, h, fmt):
+    """(library code, codes [m, h], scales) of an output; code rows start on
+    16 bytes, as w8a8_linear reads them, so a row of another length is a view
+    of a padded one."""
+    f = _Q8.get(fmt)
+    if f is None:
+        raise ValueError(f"fp4x: fmt is one of {sorted(_Q8)}, not {fmt!r}")
+    if h & 15:
+        q = torch.empty((m, (h + 15) & -16), dtype=f[1], device=x.device)[:, :h]
+    else:
+        q = torch.empty((m, h), dtype=f[1], device=x.device)
+    if f[0] == 2:
+        return 2, q, torch.empty((m, h // 32), dtype=torch.uint8, device=x.device)
+    return f[0], q, torch.empty(m, dtype=torch.float32, device=x.device)
+
+
+def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=False, residual_out=None):
+    """Root-mean-square norm of the rows of x [M, H], after the residual's
+    addition where one is given, into 8 bits, in one launch.
+
+    h = x + residual (rounded to the residual's type), v = h / sqrt(mean(h^2)
+    + eps) * (w + w_offset).  Returns (q, s) of v in `fmt`; with a residual
+    also h, the next residual (written to residual_out if given, which may be
+    the residual itself); with normed=True also v in x's type.
+
+    fmt "int8": int8 codes and fp32 scales [M] (w8a8_linear takes them);
+    "e4m3": the same with float8_e4m3fn codes; "mx8": MXFP8, float8_e4m3fn
+    codes and uint8 e8m0 scales [M, H/32].  A row (mx8: a block) with an
+    infinity or a NaN gets the scale NaN.  x is bf16, fp16 or fp32; residual
+    and w have its type or are fp32.  1 <= H <= 32768."""
+    _same_gpu(x, w, residual, residual_out)
+    x = _rows2(x, "x")
+    m, h = x.shape
+    dt = _dt(x.dtype)
+    if w.dim() != 1 or w.shape[0] != h:
+        raise ValueError(f"fp4x: the norm weight must have {h} values")
+    if w.stride(0) != 1:
+        w = w.contiguous()
+    code, q, s = _q8_out(x, m, h, fmt)
+    out = [q, s]
+    r_args = (None, 0, dt)
+    ho = y = None
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError("fp4x: the residual must have x's shape")
+        residual = _rows2(residual, "the residual")
+        r_args = (residual.data_ptr(), residual.stride(0), _dt(residual.dtype))
+        ho = residual_out
+        if ho is None:
+            ho = torch.empty((m, h), dtype=residual.dtype, device=x.device)
+        elif ho.shape != x.shape or ho.dtype != residual.dtype or (h > 1 and ho.stride(1) != 1):
+            raise ValueError("fp4x: residual_out must have the residual's shape and type and unit column stride")
+        out.append(ho)
+    elif residual_out is not None:
+        raise ValueError("fp4x: residual_out needs a residual")
+    if normed:
+        y = torch.empty((m, h), dtype=x.dtype, device=x.device)
+        out.append(y)
+    rc = _L.lib().fp4x_rms_norm_q8(x.data_ptr(), x.stride(0), dt, *r_args, w.data_ptr(), _dt(w.dtype), w_offset, eps,
+                                   m, h, code, q.data_ptr(), q.stride(0), s.data_ptr(),
+                                   *((ho.data_ptr(), ho.stride(0)) if ho is not None else (None, 0)),
+                                   *((y.data_ptr(), h) if normed else (None, 0)), _L.stream_of(x))
+    if rc != _L.OK:
+        _L.check(rc, "rms_norm_q8")
+    return tuple(out)
+
+
+def silu_mul_q8(gate, up=None, fmt="int8"):
+    """silu(gate) * up in 8 bits (q, s), as rms_norm_q8's.  gate and up are
+    [M, F] rows; without up, gate holds both halves side by side ([M, 2 F],
+    the gate first), as a fused gate and up projection leaves them."""
+    _same_gpu(gate, up)
+    gate = _rows2(gate, "gate")
+    dt = _dt(gate.dtype)
+    m, f = gate.shape
+    g, gs = gate.data_ptr(), gate.stride(0)
+    if up is None:
+        if f & 1:
+            raise ValueError("fp4x: gate and up side by side need an even number of columns")
+        f >>= 1
+        u, us = g + f * gate.element_size(), gs
+    else:
+        if up.shape != gate.shape or up.dtype != gate.dtype:
+            raise ValueError("fp4x: up must have gate's shape and type")
+        up = _rows2(up, "up")
+        u, us = up.data_ptr(), up.stride(0)
+    code, q, s = _q8_out(gate, m, f, fmt)
+    rc = _L.lib().fp4x_silu_mul_q8(g, gs, u, us, dt, m, f, code, q.data_ptr(), q.stride(0), s.data_ptr(),
+                                   _L.stream_of(gate))
+    if rc != _L.OK:
+        _L.check(rc, "silu_mul_q8")
+    return q, s
+
+
+def quantize_q8(x, fmt="int8"):
+    """The rows of x [M, H] in 8 bits (q, s), as rms_norm_q8's: activations
+    with a scale per token, or a weight with a scale per output channel."""
+    _same_gpu(x)
+    x = _rows2(x, "x")
+    m, h = x.shape
+    code, q, s = _q8_out(x, m, h, fmt)
+    rc = _L.lib().fp4x_quantize_q8(x.data_ptr(), x.stride(0), _dt(x.dtype), m, h, code, q.data_ptr(), q.stride(0),
+                                   s.data_ptr(), _L.stream_of(x))
+    if rc != _L.OK:
+        _L.check(rc, "quantize_q8")
+    return q, s
+
+
+def _codes16(q, what):
+    """int8 rows that start on 16 bytes and can be read to the next 16-byte
+    boundary past their end: q itself as the q8 functions lay it out, a copy
+    otherwise."""
+    if q.dtype != torch.int8:
+        raise TypeError(f"fp4x: {what} must be int8, got {q.dtype}")
+    if q.dim() != 2:
+        raise ValueError(f"fp4x: {what} must be 2-D")
+    n, k = q.shape
+    ld, one = q.stride()
+    if ((one == 1 or k == 1) and ld & 15 == 0 and ld >= k and q.data_ptr() & 15 == 0
+            and (k & 15 == 0 or q.storage_offset() + (n - 1) * ld + (k + 15 & -16) <= q.untyped_storage().nbytes())):
+        return q
+    c = torch.empty((n, (k + 15) & -16), dtype=torch.int8, device=q.device)[:, :k]
+    return c.copy_(q)
+
+
+def _scales(s, n, what):
+    if s.dtype != torch.float32 or s.numel() != n:
+        raise ValueError(f"fp4x: {what} must be {n} fp32 scales")
+    return s if s.is_contiguous() else s.contiguous()
+
+
+def w8a8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
+    """y[m, n] = (sum_k xq[m, k] * wq[n, k]) * xs[m] * ws[n] + bias[n]: int8
+    activations [M, K] with a scale per token, int8 weights [N, K] with a scale
+    per output channel (both as quantize_q8 makes them), the sum exact in int32.
+    Any M, N and K up to 131071; out_dtype bf16, fp16 or fp32.  Rows that do
+    not start on 16 bytes are copied first, which for a weight is worth doing
+    once (quantize_q8 lays its codes out so)."""
+    _same_gpu(xq, xs, wq, ws, bias)
+    xq, wq = _codes16(xq, "xq"), _codes16(wq, "wq")
+    m, k = xq.shape
+    n, kw = wq.shape
+    if kw != k:
+        raise ValueError(f"fp4x: activation K={k} does not match weight K={kw}")
+    xs, ws = _scales(xs, m, "xs"), _scales(ws, n, "ws")
+    b = None
+    if bias is not None:
+        if bias.shape != (n,):
+            raise ValueError(f"fp4x: the bias must have {n} values")
+        bias = bias.float().contiguous()
+        b = bias.data_ptr()
+    out = torch.empty((m, n), dtype=out_dtype, device=xq.device)
+    rc = _L.lib().fp4x_w8a8_linear(xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
+                                   ws.data_ptr(), b, out.data_ptr(), n, _dt(out_dtype), m, n, k, _L.stream_of(xq))
+    if rc != _L.OK:
+        _L.check(rc, "w8a8_linear")
+    return out
 
 
 def w8_linear_layers(x3, q3, s3, out_dtype=torch.bfloat16):
