@@ -284,12 +284,15 @@ int fp4x_quantize_q8(const void* x, int64_t x_stride, int dtype, int M, int H, i
 /* out[m, n] = cast(((sum_k xq[m, k] * wq[n, k]) * xs[m]) * ws[n] + bias[n]):
  * int8 codes, the sum exact in int32 (K <= 131071), then rounded fp32 steps, so
  * results do not depend on the launch shape.  xs fp32 [M], ws and bias (NULL:
- * none) fp32 [N].  Code rows start on 16 bytes (strides a multiple of 16) and
- * are readable to the next 16-byte boundary past K; what is there is ignored.
- * Any M, N and K.  No counterpart in the reference. */
+ * none) fp32 [N].  Code rows start on 16 bytes (strides a multiple of 16, below
+ * 2^24) and are readable to the next 16-byte boundary past K; what is there is
+ * ignored.  M and N go to 2^24, M N to 2^37.  No counterpart in the reference. */
 int fp4x_w8a8_linear(const void* xq, int64_t x_stride, const float* xs, const void* wq, int64_t w_stride,
                      const float* ws, const float* bias, void* out, int64_t out_stride, int out_dtype, int M, int N,
                      int K, void* stream);
+/* The form (0 .. 10, from 16 x 16 to 256 x 256 tiles) that fp4x_w8a8_linear
+ * takes for a size on the current device; -1 for sizes below 1. */
+int fp4x_w8a8_form(int M, int N, int K);
 
 /* Mixer down projection: split-K W8 GEMV whose last workgroup per row tile
  * writes di = bf16(sum) [M, N] and bot = bf16(sc * sigmoid(sc)) [M, lr] with

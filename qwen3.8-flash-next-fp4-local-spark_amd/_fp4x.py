@@ -49,6 +49,7 @@ _SIGS = {
     "fp4x_silu_mul_q8": ([_P, _I64, _P, _I64, _I, _I, _I, _I, _P, _I64, _P, _P], _I),
     "fp4x_quantize_q8": ([_P, _I64, _I, _I, _I, _I, _P, _I64, _P, _P], _I),
     "fp4x_w8a8_linear": ([_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _P], _I),
+    "fp4x_w8a8_form": ([_I, _I, _I], _I),
     "fp4x_hc_down": ([_P, _I64, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P], _I),
     "fp4x_hc_up": ([_P, _I64, _P, _P, _I, _P, _I64, _P, _I, _I, _I, _I, _I, _P], _I),
     "fp4x_hc_mix": ([_P, _I64, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _P, _I64, _P, _I, _I,

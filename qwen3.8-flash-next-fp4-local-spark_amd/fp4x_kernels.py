@@ -328,16 +328,16 @@ def quantize_q8(x, fmt="int8"):
 
 
 def _codes16(q, what):
-    """int8 rows that start on 16 bytes and can be read to the next 16-byte
-    boundary past their end: q itself as the q8 functions lay it out, a copy
-    otherwise."""
+    """int8 rows that start on 16 bytes, less than 2^24 apart, and can be read
+    to the next 16-byte boundary past their end: q itself as the q8 functions
+    lay it out, a copy otherwise."""
     if q.dtype != torch.int8:
         raise TypeError(f"fp4x: {what} must be int8, got {q.dtype}")
     if q.dim() != 2:
         raise ValueError(f"fp4x: {what} must be 2-D")
     n, k = q.shape
     ld, one = q.stride()
-    if ((one == 1 or k == 1) and ld & 15 == 0 and ld >= k and q.data_ptr() & 15 == 0
+    if ((one == 1 or k == 1) and ld & 15 == 0 and k <= ld < 1 << 24 and q.data_ptr() & 15 == 0
             and (k & 15 == 0 or q.storage_offset() + (n - 1) * ld + (k + 15 & -16) <= q.untyped_storage().nbytes())):
         return q
     c = torch.empty((n, (k + 15) & -16), dtype=torch.int8, device=q.device)[:, :k]

@@ -284,6 +284,46 @@ def test_linear_sizes(F, m, n, k, out):
     check_linear(F, m, n, k, out, True)
 
 
+# every form, K below and inside a unit, several tiles per workgroup
+FORMS = [(1, 640), (40, 1000), (16, 18000), (100, 1280), (64, 5200), (33, 9001), (96, 13000), (250, 13310), (256, 16384),
+         (700, 3001), (512, 16500), (1100, 16390), (4100, 4400), (9000, 70), (33, 40000), (1000, 5000)]
+FORM_KS = [100, 320, 1400, 2571]
+
+
+@pytest.mark.parametrize("k", FORM_KS)
+@pytest.mark.parametrize("m,n", FORMS)
+def test_linear_forms(F, m, n, k):
+    out, bias = ("bf16", "f16", "f32")[(m + k) % 3], m % 2 == 0
+    xq, xs = int_codes(m + k, m, k)
+    wq, ws = int_codes(m + k + 1, n, k)
+    b = torch.randn(n, generator=torch.Generator().manual_seed(m)) if bias else None
+    y = F.w8a8_linear(padded(xq), xs.cuda(), padded(wq), ws.cuda(), None if b is None else b.cuda(), DT[out])
+    rows = np.unique(np.r_[:min(m, 40), np.linspace(0, m - 1, 60).astype(int), max(0, m - 40):m])   # of large ones
+    want = o8.w8a8(xq.numpy()[rows], xs.numpy()[rows], wq.numpy(), ws.numpy(), None if b is None else b.numpy())
+    same(y[torch.from_numpy(rows).cuda()], rounder(out)(want), (m, n, k, out))
+
+
+def test_linear_forms_are_all_reached(F):
+    import _fp4x
+    form = _fp4x.lib().fp4x_w8a8_form
+    assert {form(m, n, k) for m, n in FORMS for k in FORM_KS} == set(range(11))
+    assert form(0, 1, 1) == form(1, 0, 1) == form(1, 1, 0) == -1
+
+
+def test_linear_far_rows(F):
+    """Strides up to the limit, and beyond it (copied)."""
+    xq, xs = int_codes(1, 300, 200)
+    wq, ws = int_codes(2, 50, 200)
+    want = rounder("bf16")(o8.w8a8(xq.numpy(), xs.numpy(), wq.numpy(), ws.numpy()))
+    for ld in ((1 << 24) - 16, 1 << 24):
+        big = torch.empty(299 * ld + 208, dtype=torch.int8, device="cuda")
+        x = big.as_strided((300, 200), (ld, 1))
+        x.copy_(xq)
+        same(F.w8a8_linear(x, xs.cuda(), wq.cuda(), ws.cuda()), want, ld)
+        same(F.w8a8_linear(wq.cuda(), ws.cuda(), x, xs.cuda(), out_dtype=torch.float32),
+             o8.w8a8(wq.numpy(), ws.numpy(), xq.numpy(), xs.numpy()), ld)
+
+
 def test_linear_extreme_codes(F):
     """The longest sum of the largest products fits the int32 accumulator."""
     for m, n in ((1, 16), (20, 16), (80, 32), (256, 256)):

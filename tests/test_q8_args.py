@@ -54,7 +54,8 @@ def test_linear_refusals(L):
     for kw in (dict(M=-1), dict(N=0), dict(K=0), dict(K=131072, xs=131072, ws=131072), dict(dt=3), dict(x=None),
                dict(sx=None), dict(w=None), dict(sw=None), dict(o=None), dict(x=P + 8), dict(w=P + 8), dict(xs=72),
                dict(ws=72), dict(xs=48), dict(ws=48), dict(sx=P + 2), dict(sw=P + 2), dict(b=P + 2), dict(o=P + 1),
-               dict(o=P + 2, dt=1), dict(os=47), dict(M=(1 << 24) + 1), dict(N=(1 << 24) + 1)):
+               dict(o=P + 2, dt=1), dict(os=47), dict(M=(1 << 24) + 1), dict(N=(1 << 24) + 1),
+               dict(M=1 << 20, N=1 << 18, os=1 << 18), dict(xs=1 << 24), dict(ws=1 << 24)):
         assert linear(L, **kw) == L.ERR_ARG, kw
         assert L.lib().fp4x_last_error().startswith(b"w8a8_linear")
     assert linear(L, M=0) == L.OK
