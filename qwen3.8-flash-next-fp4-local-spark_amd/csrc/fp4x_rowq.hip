@@ -38,7 +38,7 @@ enum RowFmt : int { ROW_INT8, ROW_E4M3, ROW_MX8 };
 struct RowArgs {
   const void* x;  int64_t x_stride;                // rows (the gate)
   const void* r;  int64_t r_stride;                // residual or null (the up rows)
-  const void* w;  float w_off;  double eps;        // norm weight
+  const void* w;  float w_off;  double eps, inv_h; // norm weight, 1 / H
   int M, H, fmt, L, rpb;                           // lanes per row, rows per workgroup
   uint8_t* q;  int64_t q_stride;
   void* s;
@@ -113,18 +113,52 @@ __device__ __forceinline__ float round_to(float f) {
 struct SumF64 { __device__ double operator()(double a, double b) const { return a + b; } };
 struct MaxF32 { __device__ float operator()(float a, float b) const { return __builtin_elementwise_maximum(a, b); } };
 
-// All-reduce over a row's L lanes: a butterfly within a wave, then the waves'
-// results in wave order through LDS (`slot`: a value per wave, used once
-// between barriers).
+// A value of the lane that is 1, 2, 4 or 8 lanes on within 16 (or, for 4 and
+// 8, of one that holds the same: the reductions below come to it with quads,
+// then groups of 8, alike), in registers.
+template <int S>
+__device__ __forceinline__ uint32_t lane_other(uint32_t v) {
+  constexpr int ctrl = S == 1 ? 0xB1 : S == 2 ? 0x4E : S == 4 ? 0x141 : 0x140;
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true);
+}
+template <int S, class T, class Op>
+__device__ __forceinline__ T fold(T v, Op op) {
+  struct Words { uint32_t w[sizeof(T) / 4]; } a = __builtin_bit_cast(Words, v), b;
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(T) / 4; ++i) {
+    if constexpr (S <= 8) {
+      b.w[i] = lane_other<S>(a.w[i]);
+    } else if constexpr (S == 16) {                // every lane gets both rows' (halves') values
+      const auto p = __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
+      a.w[i] = p[0];
+      b.w[i] = p[1];
+    } else {
+      const auto p = __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false);
+      a.w[i] = p[0];
+      b.w[i] = p[1];
+    }
+  }
+  return op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+}
+
+// All-reduce over a row's L lanes: a butterfly within a wave, then one over the
+// waves' results through LDS (`slot`: a value per wave, used once between
+// barriers; 0 is the operations' identity here).  With lane exchanges through
+// LDS, the waves' results read one by one, and fp64 divisions, the norm of 3
+// rows of 2560 took 4.2 us and that of 4096 24.6; now 3.35 and 22.
 template <class T, class Op>
 __device__ __forceinline__ T row_reduce(T v, int L, T* slot, Op op) {
-  const int w = L < 64 ? L : 64;
-  for (int s = 1; s < w; s <<= 1) v = op(v, __shfl_xor(v, s, 64));
+  v = fold<2>(fold<1>(v, op), op);
+  if (L > 4) v = fold<4>(v, op);
+  if (L > 8) v = fold<8>(v, op);
+  if (L > 16) v = fold<16>(v, op);
+  if (L > 32) v = fold<32>(v, op);
   if (L > 64) {
     if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = slot[0];
-    for (int i = 1; i < L >> 6; ++i) v = op(v, slot[i]);
+    const int i = threadIdx.x & 15;
+    v = i < L >> 6 ? slot[i] : T(0);
+    v = fold<8>(fold<4>(fold<2>(fold<1>(v, op), op), op), op);
   }
   return v;
 }
@@ -149,22 +183,22 @@ template <int KIND, int TX, int TR, int TW, int C>
 __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
   __shared__ double sum_slot[16];
   __shared__ float max_slot[16];
-  const int t = threadIdx.x, L = a.L, l = L < 64 ? t & (L - 1) : t, sub = L < 64 ? t / L : 0;
+  const int t = threadIdx.x, L = a.L, l = L <= 64 ? t & (L - 1) : t, sub = L <= 64 ? t / L : 0;
   const int last = a.H - 8, n = a.H < 8 ? a.H : 8;
-  for (int64_t rb = blockIdx.x; rb * a.rpb < a.M; rb += gridDim.x) {
+  const bool two = KIND == ROW_SILU || (KIND == ROW_NORM && a.r);
+  int k[C];
+  Raw8<TX> x[C];
+  Raw8<TR> r[C];
+  Raw8<TW> w[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int k0 = (c * L + l) * 8;
+    k[c] = k0 < last ? k0 : last < 0 ? 0 : last;
+  }
+  const auto load = [&](int64_t rb) __attribute__((always_inline)) {
     const int64_t want = rb * a.rpb + sub, row = want < a.M ? want : a.M - 1;
-    const bool live = want < a.M;
-    Raw8<TX> x[C];
-    Raw8<TR> r[C];
-    Raw8<TW> w[C];
-    int k[C];
-    const bool two = KIND == ROW_SILU || (KIND == ROW_NORM && a.r);
-    // every load of the row goes out first, where the registers hold it (C <= 2)
-    const auto load_w = [&](int c) {
-      if (C == 1 && n < 8) w[c].load_n(a.w, k[c], n);
-      else w[c].load(a.w, k[c]);
-    };
-    const auto load_row = [&](int c) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
       const int64_t xi = row * a.x_stride + k[c], ri = row * a.r_stride + k[c];
       if (C == 1 && n < 8) {
         x[c].load_n(a.x, xi, n);
@@ -173,26 +207,32 @@ __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
         x[c].load(a.x, xi);
         if (two) r[c].load(a.r, ri);
       }
-    };
+    }
+  };
+  if constexpr (KIND == ROW_NORM && C <= 3) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int k0 = (c * L + l) * 8;
-      k[c] = k0 < last ? k0 : last < 0 ? 0 : last;
-      if (C <= 2) {
-        load_row(c);
-        if (KIND == ROW_NORM) load_w(c);
-      }
+      if (C == 1 && n < 8) w[c].load_n(a.w, k[c], n);
+      else w[c].load(a.w, k[c]);
     }
+  }
+  for (int64_t rb = blockIdx.x; rb * a.rpb < a.M; rb += gridDim.x) {
+    const int64_t want = rb * a.rpb + sub, row = want < a.M ? want : a.M - 1;
+    const bool live = want < a.M;
+    load(rb);
     float f[C][8];
-    if constexpr (KIND == ROW_NORM) {
-      double ss = 0.0;
+    double ss = 0.0;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (C > 2) load_row(c);
-        x[c].get(f[c]);
+    for (int c = 0; c < C; ++c) {
+      x[c].get(f[c]);
+      float g[8];
+      if (two) r[c].get(g);
+      if constexpr (KIND == ROW_SILU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[c][j] = silu_f32(f[c][j]) * g[j];
+      }
+      if constexpr (KIND == ROW_NORM) {
         if (two) {
-          float g[8];
-          r[c].get(g);
 #pragma unroll
           for (int j = 0; j < 8; ++j) f[c][j] = round_to<TR>(f[c][j] + g[j]);
         }
@@ -208,33 +248,23 @@ __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
           }
         }
       }
+    }
+    if constexpr (KIND == ROW_NORM) {
       ss = row_reduce(ss, L, sum_slot, SumF64());
-      const float rs = (float)(1.0 / sqrt(ss / a.H + a.eps));
+      const float rs = (float)rsqrt(ss * a.inv_h + a.eps);
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const bool in = live && (c * L + l) * 8 < a.H;
         if (a.h && in) store8<TR>(a.h, row * a.h_stride + k[c], f[c], n);
         float g[8];
-        if (C > 2) {
+        if (C > 3) {
           asm volatile("" ::: "memory");           // one chunk's weights at a time
-          load_w(c);
+          w[c].load(a.w, k[c]);
         }
         w[c].get(g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[c][j] = (f[c][j] * rs) * (g[j] + a.w_off);
         if (a.y && in) store8<TX>(a.y, row * a.y_stride + k[c], f[c], n);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (C > 2) load_row(c);
-        x[c].get(f[c]);
-        if (KIND == ROW_SILU) {
-          float g[8];
-          r[c].get(g);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[c][j] = silu_f32(f[c][j]) * g[j];
-        }
       }
     }
 
@@ -249,8 +279,7 @@ __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float b = m[c];                            // 4 lanes hold a block of 32
-        b = __builtin_elementwise_maximum(b, __shfl_xor(b, 1, 64));
-        b = __builtin_elementwise_maximum(b, __shfl_xor(b, 2, 64));
+        b = fold<2>(fold<1>(b, MaxF32()), MaxF32());
         const bool fin = b < __builtin_inff();
         const int e = (int)(__float_as_uint(b) >> 23);
         const int X = e == 0 ? -127 : max(e - 127 - 8, -127);
@@ -272,13 +301,20 @@ __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
       amax = row_reduce(amax, L, max_slot, MaxF32());
       const bool fin = amax < __builtin_inff();
       const float s = fmaxf(amax, 1e-12f) / (a.fmt == ROW_INT8 ? 127.0f : 448.0f);
-      const bool quick = fin && mid_range(s);
+      // the rounded quotient from the reciprocal where every row of the wave allows it (a branch: the division that it
+      // saves is 10 of 16 operations per value)
+      const bool quick = __all(fin && mid_range(s));
       const float rc = 1.0f / s;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float g[8];
+        if (quick) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = quick ? exact_quot(f[c][j], s, rc) : f[c][j] / s;
+          for (int j = 0; j < 8; ++j) g[j] = exact_quot(f[c][j], s, rc);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[j] = f[c][j] / s;
+        }
         uint32_t lo, hi;
         if (a.fmt == ROW_INT8) {
           uint32_t b[8];
@@ -303,23 +339,35 @@ __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
 
 constexpr int kRowMaxH = 32768;                    // 1024 lanes of 4 chunks
 
+// Lanes per row and chunks per lane.  Rows of up to 256 values share a wave.
+// Few rows (their waves at one chunk per lane fit the CUs at 16 each) take one
+// chunk per lane, the shortest chain: 3 rows of 2560, normed, 3.35 us (2
+// chunks: 3.7).  More rows are bound by the bytes that a CU can have on their
+// way, and take 2 chunks, or 3 where that leaves no more lanes idle and 2 would
+// take more than 4 waves: 16384 rows of 2560, quantized, 25 us (1 chunk: 51, 3:
+// 27); 4096 of 6144, gated, 25.8 (1: 35, 2: 29.5); 3333 of 12000, normed, 57
+// (2: 64).  Rows loaded ahead of the one that is reduced gained nothing.
 template <int KIND, int TX, int TR, int TW>
 static int launch_row_q8(RowArgs a, hipStream_t st) {
   const int chunks = (a.H + 7) / 8;
+  const auto lanes = [&](int c) { return (chunks + 64 * c - 1) / (64 * c) * 64; };
   int C = 1;
   a.L = 4;
   if (chunks <= 32) {
     while (a.L < chunks) a.L <<= 1;
   } else {
-    while (chunks > C * 1024) C <<= 1;
-    a.L = (chunks + 64 * C - 1) / (64 * C) * 64;
+    if (chunks > 1024 || (int64_t)a.M * (lanes(1) / 64) > 16 * device_cus())
+      C = lanes(2) * 2 < lanes(3) * 3 || lanes(2) <= 256 ? 2 : 3;
+    if (lanes(C) > 1024) C = 4;
+    a.L = lanes(C);
   }
-  const int threads = a.L < 64 ? 256 : a.L;
-  a.rpb = a.L < 64 ? 256 / a.L : 1;
+  const int threads = a.L <= 64 ? 256 : a.L;
+  a.rpb = a.L <= 64 ? 256 / a.L : 1;
   const unsigned grid = (unsigned)std::min<int64_t>((a.M + (int64_t)a.rpb - 1) / a.rpb, 1 << 20);
   const dim3 g(grid), b(threads);
   if (C == 1) hipLaunchKernelGGL((row_q8_kernel<KIND, TX, TR, TW, 1>), g, b, 0, st, a);
   else if (C == 2) hipLaunchKernelGGL((row_q8_kernel<KIND, TX, TR, TW, 2>), g, b, 0, st, a);
+  else if (C == 3) hipLaunchKernelGGL((row_q8_kernel<KIND, TX, TR, TW, 3>), g, b, 0, st, a);
   else hipLaunchKernelGGL((row_q8_kernel<KIND, TX, TR, TW, 4>), g, b, 0, st, a);
   return check_launch("row_q8");
 }
@@ -357,7 +405,7 @@ int fp4x_rms_norm_q8(const void* x, int64_t x_stride, int dtype, const void* res
                      const void* w, int w_dtype, float w_offset, double eps, int M, int H, int fmt, void* q,
                      int64_t q_stride, void* s, void* res_out, int64_t res_out_stride, void* normed,
                      int64_t normed_stride, void* stream) {
-  RowArgs a{x, x_stride, res, res_stride, w, w_offset, eps, M, H, fmt, 0, 0, static_cast<uint8_t*>(q), q_stride, s,
+  RowArgs a{x, x_stride, res, res_stride, w, w_offset, eps, 1.0 / (H > 0 ? H : 1), M, H, fmt, 0, 0, static_cast<uint8_t*>(q), q_stride, s,
             res_out, res_out_stride, normed, normed_stride};
   const char* what = "rms_norm_q8";
   if (int rc = row_check(what, a, dtype)) return rc;
@@ -387,7 +435,7 @@ int fp4x_rms_norm_q8(const void* x, int64_t x_stride, int dtype, const void* res
 
 int fp4x_silu_mul_q8(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int dtype, int M, int F,
                      int fmt, void* q, int64_t q_stride, void* s, void* stream) {
-  RowArgs a{gate, gate_stride, up, up_stride, nullptr, 0.0f, 0.0, M, F, fmt, 0, 0, static_cast<uint8_t*>(q), q_stride,
+  RowArgs a{gate, gate_stride, up, up_stride, nullptr, 0.0f, 0.0, 0.0, M, F, fmt, 0, 0, static_cast<uint8_t*>(q), q_stride,
             s, nullptr, 0, nullptr, 0};
   const char* what = "silu_mul_q8";
   if (int rc = row_check(what, a, dtype)) return rc;
@@ -401,7 +449,7 @@ int fp4x_silu_mul_q8(const void* gate, int64_t gate_stride, const void* up, int6
 
 int fp4x_quantize_q8(const void* x, int64_t x_stride, int dtype, int M, int H, int fmt, void* q, int64_t q_stride,
                      void* s, void* stream) {
-  RowArgs a{x, x_stride, nullptr, 0, nullptr, 0.0f, 0.0, M, H, fmt, 0, 0, static_cast<uint8_t*>(q), q_stride, s,
+  RowArgs a{x, x_stride, nullptr, 0, nullptr, 0.0f, 0.0, 0.0, M, H, fmt, 0, 0, static_cast<uint8_t*>(q), q_stride, s,
             nullptr, 0, nullptr, 0};
   if (int rc = row_check("quantize_q8", a, dtype)) return rc;
   if (M == 0) return FP4X_OK;

@@ -226,13 +226,15 @@ def _q8_out(x, m, h, fmt):
     f = _Q8.get(fmt)
     if f is None:
         raise ValueError(f"fp4x: fmt is one of {sorted(_Q8)}, not {fmt!r}")
+    code, dtype = f
+    dev = x.device
     if h & 15:
-        q = torch.empty((m, (h + 15) & -16), dtype=f[1], device=x.device)[:, :h]
-    else:
-        q = torch.empty((m, h), dtype=f[1], device=x.device)
-    if f[0] == 2:
-        return 2, q, torch.empty((m, h // 32), dtype=torch.uint8, device=x.device)
-    return f[0], q, torch.empty(m, dtype=torch.float32, device=x.device)
+        q = torch.empty((m, (h + 15) & -16), dtype=dtype, device=dev)[:, :h]
+    else:                                           # (empty_strided: 0.4 us less than empty)
+        q = torch.empty_strided((m, h), (h, 1), dtype=dtype, device=dev)
+    if code == 2:
+        return code, q, torch.empty((m, h // 32), dtype=torch.uint8, device=dev)
+    return code, q, torch.empty_strided((m,), (1,), dtype=torch.float32, device=dev)
 
 
 def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=False, residual_out=None):
@@ -253,34 +255,36 @@ def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=
     x = _rows2(x, "x")
     m, h = x.shape
     dt = _dt(x.dtype)
-    if w.dim() != 1 or w.shape[0] != h:
+    if w.shape != (h,):
         raise ValueError(f"fp4x: the norm weight must have {h} values")
     if w.stride(0) != 1:
         w = w.contiguous()
     code, q, s = _q8_out(x, m, h, fmt)
     out = [q, s]
-    r_args = (None, 0, dt)
-    ho = y = None
+    rp = hp = yp = None
+    rs = hs = 0
+    rdt = dt
     if residual is not None:
         if residual.shape != x.shape:
             raise ValueError("fp4x: the residual must have x's shape")
         residual = _rows2(residual, "the residual")
-        r_args = (residual.data_ptr(), residual.stride(0), _dt(residual.dtype))
+        rp, rs, rdt = residual.data_ptr(), residual.stride(0), _dt(residual.dtype)
         ho = residual_out
         if ho is None:
-            ho = torch.empty((m, h), dtype=residual.dtype, device=x.device)
+            ho = torch.empty_strided((m, h), (h, 1), dtype=residual.dtype, device=x.device)
         elif ho.shape != x.shape or ho.dtype != residual.dtype or (h > 1 and ho.stride(1) != 1):
             raise ValueError("fp4x: residual_out must have the residual's shape and type and unit column stride")
+        hp, hs = ho.data_ptr(), ho.stride(0)
         out.append(ho)
     elif residual_out is not None:
         raise ValueError("fp4x: residual_out needs a residual")
     if normed:
-        y = torch.empty((m, h), dtype=x.dtype, device=x.device)
+        y = torch.empty_strided((m, h), (h, 1), dtype=x.dtype, device=x.device)
+        yp = y.data_ptr()
         out.append(y)
-    rc = _L.lib().fp4x_rms_norm_q8(x.data_ptr(), x.stride(0), dt, *r_args, w.data_ptr(), _dt(w.dtype), w_offset, eps,
-                                   m, h, code, q.data_ptr(), q.stride(0), s.data_ptr(),
-                                   *((ho.data_ptr(), ho.stride(0)) if ho is not None else (None, 0)),
-                                   *((y.data_ptr(), h) if normed else (None, 0)), _L.stream_of(x))
+    rc = _L.lib().fp4x_rms_norm_q8(x.data_ptr(), x.stride(0), dt, rp, rs, rdt, w.data_ptr(), _dt(w.dtype), w_offset,
+                                   eps, m, h, code, q.data_ptr(), q.stride(0), s.data_ptr(), hp, hs, yp, h,
+                                   _L.stream_of(x))
     if rc != _L.OK:
         _L.check(rc, "rms_norm_q8")
     return tuple(out)
@@ -370,7 +374,7 @@ def w8a8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
             raise ValueError(f"fp4x: the bias must have {n} values")
         bias = bias.float().contiguous()
         b = bias.data_ptr()
-    out = torch.empty((m, n), dtype=out_dtype, device=xq.device)
+    out = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=xq.device)
     rc = _L.lib().fp4x_w8a8_linear(xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0),
                                    ws.data_ptr(), b, out.data_ptr(), n, _dt(out_dtype), m, n, k, _L.stream_of(xq))
     if rc != _L.OK:
