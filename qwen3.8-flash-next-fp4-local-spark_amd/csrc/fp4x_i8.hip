@@ -242,7 +242,7 @@ struct I8Tile {
                 BN % 64 == 0 && NI <= 2 && S >= 2, "tile");
 };
 
-template <int BM, int BN, int WM, int WN, int S>
+template <int BM, int BN, int WM, int WN, int S, bool TAIL>
 __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a) {
   using C = I8Tile<BM, BN, WM, WN, S>;
   constexpr int MI = C::MI, NI = C::NI, NL = C::NL, NM = MI * NI, NR = MI + NI;
@@ -253,8 +253,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
   const int stride = (gridDim.x + 7 - xcd) >> 3;   // workgroups of this XCD
   const int first = run.first + (blockIdx.x >> 3), tiles = (run.count - (blockIdx.x >> 3) + stride - 1) / stride;
   const int kts = (a.K + 127) >> 7, V = tiles * kts;
-  const bool tail = a.K & 127;
-  const int last = (a.K - 1) >> 4;
+  const int last = (a.K - 1) >> 4;                 // TAIL: K ends inside a k-tile
 
   // ---- the loads: k-tile lk of tile lt
   // LDS row r holds chunk c of its 128 bytes at c ^ key: the 16 lanes that LDS serves together read different banks
@@ -304,7 +303,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
       lk = 0;
       if (++lt < tiles) next_tile();
     }
-    if (tail && lk == kts - 1) clamp_tail();       // (next_tile sets the offsets anew)
+    if (TAIL && lk == kts - 1) clamp_tail();       // (next_tile sets the offsets anew)
   };
 
   // ---- the products
@@ -331,7 +330,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
   const auto step = [&](int kk, bool more, int so, bool fill, int fo) __attribute__((always_inline)) {
     const int b = kk & 1;
     int q = 0, j = 0;
-    if (tail && ek == kts - 1) {
+    if (TAIL && ek == kts - 1) {
 #pragma unroll
       for (int s = 0; s < MI; ++s) x[b][s] = keep_to(x[b][s], ek * 8 + kk * 2 + h, a.K);
     }
@@ -411,7 +410,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
   };
 
   next_tile();
-  if (tail && kts == 1) clamp_tail();
+  if (TAIL && kts == 1) clamp_tail();
 #pragma unroll
   for (int d = 0; d < S; ++d)
     if (d < V) {
@@ -484,6 +483,13 @@ constexpr I8Form kI8Forms[] = {
     {128, 128, 2, 0, 2, 3.21f, 1.37f, 0.552f}, {256, 128, 1, 0, 3, 0.19f, 5.48f, 0.676f},
     {256, 256, 1, 0, 2, 0.11f, 7.94f, 1.259f}};
 
+template <int BM, int BN, int WM, int WN, int S>
+static void launch_i8_tile(dim3 grid, const I8Args& a, hipStream_t st) {
+  const dim3 threads(64 * WM * WN);
+  if (a.K & 127) hipLaunchKernelGGL((i8_tile_kernel<BM, BN, WM, WN, S, true>), grid, threads, 0, st, a);
+  else hipLaunchKernelGGL((i8_tile_kernel<BM, BN, WM, WN, S, false>), grid, threads, 0, st, a);
+}
+
 template <int F>
 static void launch_i8(I8Args a, hipStream_t st) {
   constexpr I8Form f = kI8Forms[F];
@@ -498,12 +504,12 @@ static void launch_i8(I8Args a, hipStream_t st) {
   else if constexpr (F == 2) hipLaunchKernelGGL((i8_ring_kernel<1, 4, 4, 2>), grid, dim3(256), 0, st, a);
   else if constexpr (F == 3) hipLaunchKernelGGL((i8_ring_kernel<2, 2, 4, 2>), grid, dim3(256), 0, st, a);
   else if constexpr (F == 4) hipLaunchKernelGGL((i8_ring_kernel<2, 4, 4, 2>), grid, dim3(256), 0, st, a);
-  else if constexpr (F == 5) hipLaunchKernelGGL((i8_tile_kernel<64, 64, 2, 2, 4>), grid, dim3(256), 0, st, a);
-  else if constexpr (F == 6) hipLaunchKernelGGL((i8_tile_kernel<64, 128, 2, 2, 3>), grid, dim3(256), 0, st, a);
-  else if constexpr (F == 7) hipLaunchKernelGGL((i8_tile_kernel<128, 128, 2, 4, 4>), grid, dim3(512), 0, st, a);
-  else if constexpr (F == 8) hipLaunchKernelGGL((i8_tile_kernel<128, 128, 2, 2, 2>), grid, dim3(256), 0, st, a);
-  else if constexpr (F == 9) hipLaunchKernelGGL((i8_tile_kernel<256, 128, 4, 2, 3>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((i8_tile_kernel<256, 256, 2, 4, 2>), grid, dim3(512), 0, st, a);
+  else if constexpr (F == 5) launch_i8_tile<64, 64, 2, 2, 4>(grid, a, st);
+  else if constexpr (F == 6) launch_i8_tile<64, 128, 2, 2, 3>(grid, a, st);
+  else if constexpr (F == 7) launch_i8_tile<128, 128, 2, 4, 4>(grid, a, st);
+  else if constexpr (F == 8) launch_i8_tile<128, 128, 2, 2, 2>(grid, a, st);
+  else if constexpr (F == 9) launch_i8_tile<256, 128, 4, 2, 3>(grid, a, st);
+  else launch_i8_tile<256, 256, 2, 4, 2>(grid, a, st);
 }
 
 static int choose_i8(int M, int N, int K) {
