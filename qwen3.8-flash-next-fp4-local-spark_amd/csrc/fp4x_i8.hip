@@ -469,19 +469,20 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
 // 150 sizes (1 to 4096 rows by [2560 x 640], [640 x 2560], [64 x 2560],
 // [1280 x 2560], [16384 x 2560], [2560 x 6144], [4096 x 4096], [512 x 10240],
 // [10000 x 1280], [18000 x 256], weights from HBM); the form with the least
-// estimate takes 1.2% more than the fastest on average (geometric), 21% at
+// estimate takes 0.9% more than the fastest on average (geometric), 21% at
 // most.  Leaving any one form out costs 1.5 to 2.9%, up to 41% on one size,
-// but for 64 x 64 tiles in the ring (no loss), which are left out.
+// but for 64 x 64 tiles in the ring (no loss on average, 10% on one size),
+// which are left out.
 constexpr int64_t kI8MaxStride = (1 << 24) - 16;   // 256 rows within 32-bit offsets
 
 struct I8Form { int bm, bn, slots, ring, stages; float a, b, d; };
 constexpr I8Form kI8Forms[] = {
-    {16, 16, 2, 1, 2, 1.69f, 0.60f, 0.043f},   {16, 32, 2, 1, 3, 1.73f, 0.65f, 0.067f},
+    {16, 16, 2, 1, 2, 1.68f, 0.61f, 0.042f},   {16, 32, 2, 1, 3, 1.73f, 0.66f, 0.066f},
     {16, 64, 2, 1, 2, 1.79f, 0.81f, 0.108f},   {32, 32, 2, 1, 2, 1.62f, 0.82f, 0.087f},
-    {32, 64, 1, 1, 2, 0.56f, 2.54f, 0.138f},   {64, 64, 2, 0, 4, 2.78f, 0.70f, 0.220f},
-    {64, 128, 2, 0, 3, 3.04f, 1.08f, 0.326f},  {128, 128, 1, 0, 4, 0.82f, 3.49f, 0.452f},
-    {128, 128, 2, 0, 2, 3.21f, 1.37f, 0.552f}, {256, 128, 1, 0, 3, 0.19f, 5.48f, 0.676f},
-    {256, 256, 1, 0, 2, 0.11f, 7.94f, 1.259f}};
+    {32, 64, 1, 1, 2, 0.55f, 2.54f, 0.139f},   {64, 64, 2, 0, 4, 2.75f, 0.69f, 0.223f},
+    {64, 128, 2, 0, 3, 3.09f, 1.04f, 0.336f},  {128, 128, 1, 0, 4, 0.96f, 3.15f, 0.453f},
+    {128, 128, 2, 0, 2, 3.15f, 1.38f, 0.564f}, {256, 128, 1, 0, 3, 0.34f, 5.29f, 0.710f},
+    {256, 256, 1, 0, 2, 1.02f, 7.51f, 1.270f}};
 
 template <int BM, int BN, int WM, int WN, int S>
 static void launch_i8_tile(dim3 grid, const I8Args& a, hipStream_t st) {
@@ -506,7 +507,7 @@ static void launch_i8(I8Args a, hipStream_t st) {
   else if constexpr (F == 4) hipLaunchKernelGGL((i8_ring_kernel<2, 4, 4, 2>), grid, dim3(256), 0, st, a);
   else if constexpr (F == 5) launch_i8_tile<64, 64, 2, 2, 4>(grid, a, st);
   else if constexpr (F == 6) launch_i8_tile<64, 128, 2, 2, 3>(grid, a, st);
-  else if constexpr (F == 7) launch_i8_tile<128, 128, 2, 4, 4>(grid, a, st);
+  else if constexpr (F == 7) launch_i8_tile<128, 128, 4, 2, 4>(grid, a, st);
   else if constexpr (F == 8) launch_i8_tile<128, 128, 2, 2, 2>(grid, a, st);
   else if constexpr (F == 9) launch_i8_tile<256, 128, 4, 2, 3>(grid, a, st);
   else launch_i8_tile<256, 256, 2, 4, 2>(grid, a, st);

@@ -230,7 +230,7 @@ def _q8_out(m, h, fmt, dev):
     ld = h
     if h & 15:
         ld = (h + 15) & -16
-        q = torch.empty((m, ld), dtype=dtype, device=dev)[:, :h]
+        q = _new((m, ld), (ld, 1), dtype=dtype, device=dev)[:, :h]
     else:
         q = _new((m, h), (h, 1), dtype=dtype, device=dev)
     if code == 2:

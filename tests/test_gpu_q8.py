@@ -106,6 +106,31 @@ def test_norm_many_rows(F):
     assert bool((s[:-1] == float(np.float32(1.0) / np.float32(127))).all())
 
 
+# 2, 3 and 4 chunks of 8 per lane: with few rows only rows past 8192 values take those
+MANY = [(2100, 520), (1500, 1025), (700, 2571), (430, 6144), (400, 6145), (300, 8191), (280, 12000), (130, 32766)]
+
+
+@pytest.mark.parametrize("m,h", MANY)
+def test_many_rows(F, m, h):
+    r = rows(h + 2, m, h, "f32")
+    for xdt, rdt, fmt in (("bf16", "bf16", "int8"), ("f16", "f32", "e4m3"), ("f32", "f32", "int8")):
+        x, w = rows(h, m, h, xdt), (1 + 0.3 * rows(h + 1, 1, h, "f32")[0]).to(DT[xdt])
+        check_norm(F, x, w, r.to(DT[rdt]), fmt, rdt=rdt, xdt=xdt)
+        q, s = F.quantize_q8(x.cuda(), fmt)
+        a, b = codes_of(x, fmt)
+        same(q, a, "codes")
+        same(s, b, "scales")
+        # the gate and the up rows change no row but their own, whatever the number of rows
+        q, s = F.silu_mul_q8(x.cuda(), r.to(x.dtype).cuda(), fmt)
+        for i in (0, m // 2, m - 1):
+            q1, s1 = F.silu_mul_q8(x[i:i + 1].cuda(), r[i:i + 1].to(x.dtype).cuda(), fmt)
+            same(q[i:i + 1], host(q1), i)
+            same(s[i:i + 1], host(s1), i)
+    if h % 32 == 0:
+        x = rows(h, m, h, "bf16")
+        check_norm(F, x, (1 + 0.3 * rows(h + 1, 1, h, "f32")[0]).bfloat16(), None, "mx8")
+
+
 def test_norm_strides_and_alignment(F):
     base = rows(7, 6, 700, "bf16")
     w = (1 + 0.3 * rows(8, 1, 701, "f32")[0]).bfloat16()
@@ -324,6 +349,23 @@ def test_linear_far_rows(F):
              o8.w8a8(wq.numpy(), ws.numpy(), xq.numpy(), xs.numpy()), ld)
 
 
+def test_linear_far_rows_of_a_large_tile(F):
+    """Rows of one tile more than 2^31 bytes apart (18 GB of rows)."""
+    m, n, k, ld = 1100, 16390, 1400, (1 << 24) - 16
+    import _fp4x
+    assert _fp4x.lib().fp4x_w8a8_form(m, n, k) == 9  # 256 rows
+    xq, xs = int_codes(1, m, k)
+    wq, ws = int_codes(2, n, k)
+    big = torch.empty((m - 1) * ld + 1408, dtype=torch.int8, device="cuda")
+    x = big.as_strided((m, k), (ld, 1))
+    x.copy_(xq)
+    y = F.w8a8_linear(x, xs.cuda(), padded(wq), ws.cuda())
+    pick = np.r_[0:20, 240:270, 1020:1100]
+    want = rounder("bf16")(o8.w8a8(xq.numpy()[pick], xs.numpy()[pick], wq.numpy(), ws.numpy()))
+    same(y[torch.from_numpy(pick).cuda()], want, ld)
+    del big, x
+
+
 def test_linear_extreme_codes(F):
     """The longest sum of the largest products fits the int32 accumulator."""
     for m, n in ((1, 16), (20, 16), (80, 32), (256, 256)):
@@ -471,3 +513,22 @@ def test_refusals_on_device(F):
                                    torch.ones((1, 131072), dtype=torch.int8, device="cuda"), s[:1]), ValueError)):
         with pytest.raises(err):
             call()
+
+
+@pytest.mark.parametrize("tokens", [1, 37, 1024])
+def test_example_block(F, tokens):
+    """examples/mlp_w8a8.py against the block in fp32.  int8 codes are off by at most half a step of amax / 127: an rms of
+    0.29 / 127 amax, and a row of 2560 (640) normal values has amax of about 3.6 (3.2) sigma, so each quantized operand
+    adds 0.8% (0.7%) of noise: twice for the first product (inputs and weights: 1.2%), which its gate and its square
+    term pass on at most doubled, and twice for the second (1.1%): 2.7%.  Rows and channels vary: 4%."""
+    import importlib.util
+    import os
+    spec = importlib.util.spec_from_file_location(
+        "mlp_w8a8", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "mlp_w8a8.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    weights, x, residual = ex.make(tokens, seed=tokens)
+    y, h = ex.GatedMLP(*weights)(x, residual)
+    want, h32 = ex.reference(x, residual, *weights)
+    assert torch.equal(h, h32)
+    assert float((y.float() - want).norm() / want.norm()) < 0.04
