@@ -5,6 +5,7 @@ is imported first so the library binds to the HIP runtime torch already
 loaded (both use the soname libamdhip64.so.7) and shares its streams.
 """
 import ctypes
+import importlib.util
 import os
 
 import torch  # noqa: F401  (HIP runtime first)
@@ -65,6 +66,24 @@ _SIGS = {
 ABI_VERSION = 14
 
 _LIB = None
+_HOST = None
+
+
+def host():
+    """The compiled host side of eager calls (raises if it has not been built)."""
+    global _HOST
+    if _HOST is None:
+        lib()
+        path = os.path.join(HERE, "_fp4x_host.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"fp4x: {path} is not built; run build.py (hipcc, gfx950)")
+        spec = importlib.util.spec_from_file_location("_fp4x_host", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        if mod.ABI_VERSION != ABI_VERSION:
+            raise RuntimeError("fp4x: _fp4x_host.so ABI version mismatch; rebuild")
+        _HOST = mod
+    return _HOST
 
 
 def lib():

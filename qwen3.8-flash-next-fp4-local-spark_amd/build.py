@@ -1,20 +1,24 @@
-"""Builds libfp4x.so (the HIP kernels and their C ABI) in-tree for gfx950.
+"""Builds libfp4x.so (the HIP kernels and their C ABI) and _fp4x_host.so (the
+compiled host side of some eager calls) in-tree for gfx950.
 
-    python build.py            # compile every csrc/*.hip, link libfp4x.so
+    python build.py            # compile every csrc/*.hip, link libfp4x.so, then csrc/fp4x_host.cpp
 
-Each translation unit compiles in its own hipcc process; the objects and the
-library land next to this file (csrc/_build/ and libfp4x.so).
+Each translation unit compiles in a process of its own; the objects and the
+libraries land next to this file (csrc/_build/, libfp4x.so, _fp4x_host.so).
 """
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_build")
 LIB = os.path.join(HERE, "libfp4x.so")
+HOST = os.path.join(HERE, "_fp4x_host.so")
 ARCH = os.environ.get("FP4X_ARCH", "gfx950")
 
 FLAGS = [
@@ -35,6 +39,31 @@ def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
+def _host_object():
+    """Compiles csrc/fp4x_host.cpp against the installed torch's headers."""
+    src, obj = os.path.join(CSRC, "fp4x_host.cpp"), os.path.join(OBJ, "fp4x_host.o")
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    inc = os.path.join(torch, "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-c", src, "-o", obj,
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{inc}",
+           f"-I{os.path.join(inc, 'torch', 'csrc', 'api', 'include')}", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{os.path.join(os.environ.get('ROCM_PATH', '/opt/rocm'), 'include')}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {src}:\n{r.stderr[-6000:]}")
+    return obj, os.path.join(torch, "lib")
+
+
+def _link_host(obj, torch_lib):
+    tmp = HOST + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-fPIC", "-o", tmp, obj, f"-L{torch_lib}", "-lc10", "-lc10_hip",
+           "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", f"-L{HERE}", "-l:libfp4x.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
+    os.replace(tmp, HOST)
+
+
 def build(verbose=False, jobs=None):
     hipcc = _hipcc()
     if hipcc is None:
@@ -52,14 +81,17 @@ def build(verbose=False, jobs=None):
             print(f"[fp4x build] {os.path.basename(src)}", flush=True)
         return obj
 
-    with ThreadPoolExecutor(max_workers=jobs or min(8, len(srcs))) as ex:
+    with ThreadPoolExecutor(max_workers=jobs or min(8, len(srcs) + 1)) as ex:
+        host = ex.submit(_host_object)
         objs = list(ex.map(compile_one, srcs))
+        host = host.result()
     tmp = LIB + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
     os.replace(tmp, LIB)
+    _link_host(*host)
     return LIB
 
 

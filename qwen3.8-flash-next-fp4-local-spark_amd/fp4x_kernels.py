@@ -199,45 +199,7 @@ def nv4_linear(x2, wp, s, gs, cfg=(32, 256, 4), out_dtype=torch.bfloat16):
 
 
 # ----------------------------------------------------------------- 8-bit activations
-# fmt -> (the library's code, the codes' dtype)
-_Q8 = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn), "mx8": (2, torch.float8_e4m3fn)}
-_new = torch.empty_strided                           # 0.4 us less than torch.empty
-
-
-def _other_gpu():
-    raise RuntimeError("fp4x: HIP kernels need GPU tensors, all on one GPU")
-
-
-def _rows2(t, what):
-    """(rows, row stride) of a 2-D tensor; copied where its column stride is
-    not 1."""
-    if t.dim() != 2:
-        raise ValueError(f"fp4x: {what} must be 2-D")
-    ld, one = t.stride()
-    if one == 1 or t.shape[1] == 1:
-        return t, ld
-    return t.contiguous(), t.shape[1]
-
-
-def _q8_out(m, h, fmt, dev):
-    """(library code, codes [m, h], their row stride, scales) of an output;
-    code rows start on 16 bytes, as w8a8_linear reads them, so a row of another
-    length is a view of a padded one."""
-    f = _Q8.get(fmt)
-    if f is None:
-        raise ValueError(f"fp4x: fmt is one of {sorted(_Q8)}, not {fmt!r}")
-    code, dtype = f
-    ld = h
-    if h & 15:
-        ld = (h + 15) & -16
-        q = _new((m, ld), (ld, 1), dtype=dtype, device=dev)[:, :h]
-    else:
-        q = _new((m, h), (h, 1), dtype=dtype, device=dev)
-    if code == 2:
-        return code, q, ld, torch.empty((m, h // 32), dtype=torch.uint8, device=dev)
-    return code, q, ld, _new((m,), (1,), dtype=torch.float32, device=dev)
-
-
+# These functions' checks, outputs and calls are compiled (csrc/fp4x_host.cpp).
 def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=False, residual_out=None):
     """Root-mean-square norm of the rows of x [M, H], after the residual's
     addition where one is given, into 8 bits, in one launch.
@@ -252,119 +214,20 @@ def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=
     codes and uint8 e8m0 scales [M, H/32].  A row (mx8: a block) with an
     infinity or a NaN gets the scale NaN.  x is bf16, fp16 or fp32; residual
     and w have its type or are fp32.  1 <= H <= 32768."""
-    gpu = x.get_device()
-    if gpu < 0 or w.get_device() != gpu:
-        _other_gpu()
-    x, ld = _rows2(x, "x")
-    m, h = shape = x.shape
-    dt = _dt(x.dtype)
-    if w.shape != (h,):
-        raise ValueError(f"fp4x: the norm weight must have {h} values")
-    if w.stride(0) != 1:
-        w = w.contiguous()
-    dev = x.device
-    code, q, ldq, s = _q8_out(m, h, fmt, dev)
-    out = [q, s]
-    rp = hp = yp = None
-    ldr = ldh = 0
-    rdt = dt
-    if residual is not None:
-        if residual.shape != shape:
-            raise ValueError("fp4x: the residual must have x's shape")
-        residual, ldr = _rows2(residual, "the residual")
-        rdt = _dt(residual.dtype)
-        rp = residual.data_ptr()
-        ho = residual_out
-        if ho is None:
-            ho, ldh = _new((m, h), (h, 1), dtype=residual.dtype, device=dev), h
-        else:
-            if ho.shape != shape or ho.dtype != residual.dtype or (h > 1 and ho.stride(1) != 1):
-                raise ValueError("fp4x: residual_out must have the residual's shape and type and unit column stride")
-            ldh = ho.stride(0)
-        if residual.get_device() != gpu or ho.get_device() != gpu:
-            _other_gpu()
-        hp = ho.data_ptr()
-        out.append(ho)
-    elif residual_out is not None:
-        raise ValueError("fp4x: residual_out needs a residual")
-    if normed:
-        y = _new((m, h), (h, 1), dtype=x.dtype, device=dev)
-        yp = y.data_ptr()
-        out.append(y)
-    rc = _L.lib().fp4x_rms_norm_q8(x.data_ptr(), ld, dt, rp, ldr, rdt, w.data_ptr(), _dt(w.dtype), w_offset, eps, m, h,
-                                   code, q.data_ptr(), ldq, s.data_ptr(), hp, ldh, yp, h, _L.stream_of(x))
-    if rc:
-        _L.check(rc, "rms_norm_q8")
-    return tuple(out)
+    return _L.host().rms_norm_q8(x, w, eps, residual, fmt, w_offset, normed, residual_out)
 
 
 def silu_mul_q8(gate, up=None, fmt="int8"):
     """silu(gate) * up in 8 bits (q, s), as rms_norm_q8's.  gate and up are
     [M, F] rows; without up, gate holds both halves side by side ([M, 2 F],
     the gate first), as a fused gate and up projection leaves them."""
-    gpu = gate.get_device()
-    if gpu < 0 or (up is not None and up.get_device() != gpu):
-        _other_gpu()
-    gate, ldg = _rows2(gate, "gate")
-    dt = _dt(gate.dtype)
-    m, f = gate.shape
-    g = gate.data_ptr()
-    if up is None:
-        if f & 1:
-            raise ValueError("fp4x: gate and up side by side need an even number of columns")
-        f >>= 1
-        u, ldu = g + f * gate.element_size(), ldg
-    else:
-        if up.shape != gate.shape or up.dtype != gate.dtype:
-            raise ValueError("fp4x: up must have gate's shape and type")
-        up, ldu = _rows2(up, "up")
-        u = up.data_ptr()
-    code, q, ldq, s = _q8_out(m, f, fmt, gate.device)
-    rc = _L.lib().fp4x_silu_mul_q8(g, ldg, u, ldu, dt, m, f, code, q.data_ptr(), ldq, s.data_ptr(), _L.stream_of(gate))
-    if rc:
-        _L.check(rc, "silu_mul_q8")
-    return q, s
+    return _L.host().silu_mul_q8(gate, up, fmt)
 
 
 def quantize_q8(x, fmt="int8"):
     """The rows of x [M, H] in 8 bits (q, s), as rms_norm_q8's: activations
     with a scale per token, or a weight with a scale per output channel."""
-    if x.get_device() < 0:
-        _other_gpu()
-    x, ld = _rows2(x, "x")
-    m, h = x.shape
-    code, q, ldq, s = _q8_out(m, h, fmt, x.device)
-    rc = _L.lib().fp4x_quantize_q8(x.data_ptr(), ld, _dt(x.dtype), m, h, code, q.data_ptr(), ldq, s.data_ptr(),
-                                   _L.stream_of(x))
-    if rc:
-        _L.check(rc, "quantize_q8")
-    return q, s
-
-
-def _codes16(q, what):
-    """(rows, pointer, row stride) of int8 rows that start on 16 bytes, less
-    than 2^24 apart, and can be read to the next 16-byte boundary past their
-    end: q itself as the q8 functions lay it out, a copy otherwise."""
-    if q.dtype != torch.int8:
-        raise TypeError(f"fp4x: {what} must be int8, got {q.dtype}")
-    if q.dim() != 2:
-        raise ValueError(f"fp4x: {what} must be 2-D")
-    n, k = q.shape
-    ld, one = q.stride()
-    p = q.data_ptr()
-    if ((ld | p) & 15 == 0 and (one == 1 or k == 1) and k <= ld < 1 << 24
-            and (k & 15 == 0 or q.storage_offset() + (n - 1) * ld + (k + 15 & -16) <= q.untyped_storage().nbytes())):
-        return q, p, ld
-    ld = (k + 15) & -16
-    c = torch.empty((n, ld), dtype=torch.int8, device=q.device)[:, :k]
-    c.copy_(q)
-    return c, c.data_ptr(), ld
-
-
-def _scales(s, n, what):
-    if s.dtype != torch.float32 or s.numel() != n:
-        raise ValueError(f"fp4x: {what} must be {n} fp32 scales")
-    return s if s.is_contiguous() else s.contiguous()
+    return _L.host().quantize_q8(x, fmt)
 
 
 def w8a8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
@@ -374,30 +237,7 @@ def w8a8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
     Any M, N and K up to 131071; out_dtype bf16, fp16 or fp32.  Rows that do
     not start on 16 bytes are copied first, which for a weight is worth doing
     once (quantize_q8 lays its codes out so)."""
-    gpu = xq.get_device()
-    if gpu < 0 or not gpu == wq.get_device() == xs.get_device() == ws.get_device():
-        _other_gpu()
-    (xq, xp, ldx), (wq, wp, ldw) = _codes16(xq, "xq"), _codes16(wq, "wq")
-    m, k = xq.shape
-    n, kw = wq.shape
-    if kw != k:
-        raise ValueError(f"fp4x: activation K={k} does not match weight K={kw}")
-    xs, ws = _scales(xs, m, "xs"), _scales(ws, n, "ws")
-    b = None
-    if bias is not None:
-        if bias.get_device() != gpu:
-            _other_gpu()
-        if bias.shape != (n,):
-            raise ValueError(f"fp4x: the bias must have {n} values")
-        bias = bias.float().contiguous()
-        b = bias.data_ptr()
-    odt = _dt(out_dtype)
-    out = _new((m, n), (n, 1), dtype=out_dtype, device=xq.device)
-    rc = _L.lib().fp4x_w8a8_linear(xp, ldx, xs.data_ptr(), wp, ldw, ws.data_ptr(), b, out.data_ptr(), n, odt, m, n, k,
-                                   _L.stream_of(xq))
-    if rc:
-        _L.check(rc, "w8a8_linear")
-    return out
+    return _L.host().w8a8_linear(xq, xs, wq, ws, bias, out_dtype)
 
 
 def w8_linear_layers(x3, q3, s3, out_dtype=torch.bfloat16):
