@@ -39,9 +39,17 @@ struct I8Run {
                                          count((tiles >> 3) + (xcd < (tiles & 7))) {}
 };
 __device__ __forceinline__ void i8_place(const I8Args& a, int id, int bm, int bn, int& m0, int& n0) {
-  const int per = a.gm * a.nt, band = id / per, r = id % per, h = min(a.gm, a.mt - band * a.gm);
-  m0 = (band * a.gm + r % h) * bm;
-  n0 = r / h * bn;
+  int band = 0, r = id, h = a.mt;
+  if (a.mt > a.gm) {
+    const int per = a.gm * a.nt;
+    band = id / per;
+    r = id - band * per;
+    h = min(a.gm, a.mt - band * a.gm);
+  }
+  // (no general division for the heights of a band and of few rows)
+  const int n = h == 1 ? r : h == 2 ? r >> 1 : h == 3 ? (int)__umulhi(r, 0x55555556u) : h == 4 ? r >> 2 : r / h;
+  m0 = (band * a.gm + r - n * h) * bm;
+  n0 = n * bn;
 }
 
 // Direct loads to LDS: lane l's 16 (4) bytes at base + off land at lds + 16 l
@@ -77,14 +85,36 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16;
 }
 
-// Four neighbouring columns [n, n + 4) of row m; columns from N on are left out.
-__device__ __forceinline__ void i8_store4(const I8Args& a, int64_t m, int n, i32x4_t acc, float sx) {
+// Scales and bias of four neighbouring columns [n, n + 4) of row m.
+struct I8Scales {
+  float sx, sw[4], b[4];
+  __device__ __forceinline__ void load(const I8Args& a, int m, int n) {
+    sx = a.sx[min(m, a.M - 1)];
+    if (n + 4 <= a.N) {
+      get(sw, a.sw + n);
+      if (a.bias) get(b, a.bias + n);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int nj = min(n + j, a.N - 1);
+        sw[j] = a.sw[nj];
+        if (a.bias) b[j] = a.bias[nj];
+      }
+    }
+  }
+  static __device__ __forceinline__ void get(float (&f)[4], const float* p) {
+    const u32x4_a4 v = *reinterpret_cast<const u32x4_a4*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(v[j]);
+  }
+};
+// Those columns of y; the ones from N on are left out.
+__device__ __forceinline__ void i8_store4(const I8Args& a, int64_t m, int n, i32x4_t acc, const I8Scales& s) {
   float v[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int nj = n + j < a.N ? n + j : a.N - 1;
-    v[j] = ((float)acc[j] * sx) * a.sw[nj];
-    if (a.bias) v[j] = v[j] + a.bias[nj];
+    v[j] = ((float)acc[j] * s.sx) * s.sw[j];
+    if (a.bias) v[j] = v[j] + s.b[j];
   }
   const int64_t at = m * a.out_stride + n;
   if (n + 4 > a.N) {
@@ -113,12 +143,14 @@ __device__ __forceinline__ void i8_store4(const I8Args& a, int64_t m, int n, i32
 // What bounds it: the bytes a CU can have on their way.  The same split with
 // loads into registers (16 rows x 64 bytes a load, in the layout that the MFMA
 // takes) takes 14.3 us at 16 x [16384 x 2560] and 13.1 at 64 x [2560 x 6144];
-// this takes 9.9 and 7.0.
+// this takes 9.8 and 7.1 (weights from HBM).  Scales that are loaded after the
+// sums, and sums through atomics on a cleared block of LDS, took 0.6 us more.
 template <int MT, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void i8_ring_kernel(const I8Args a) {
   constexpr int R = 16 * (MT + NT), NL = R / 8, STAGE = R * 128;
   constexpr int LD = 16 * NT + 4;                  // (a row of sums starts on 16 bytes)
-  static_assert(W * D * STAGE >= 16 * MT * LD * 4, "the sums reuse the ring");
+  constexpr int ITEMS = (64 * MT * NT + 64 * W - 1) / (64 * W);   // of four columns, per thread
+  static_assert(D * STAGE >= 16 * MT * LD * 4, "the sums reuse the ring");
   __shared__ __attribute__((aligned(1024))) char lds[W * D * STAGE];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 15, g = lane >> 4;
   const I8Run run(a.mt * a.nt, blockIdx.x & 7);
@@ -152,6 +184,13 @@ __global__ __launch_bounds__(64 * W) void i8_ring_kernel(const I8Args a) {
 #pragma unroll
     for (int j = NL - 1; j >= 0; --j) i8_load16(base + s * STAGE + j * 1024, off[j], (j < 2 * MT ? xb : wb) + u * 128);
   };
+  // the epilogue's scales, before the units: a wait for a unit is then one for them too
+  I8Scales sc[ITEMS];
+#pragma unroll
+  for (int p = 0; p < ITEMS; ++p) {
+    const int e = t + p * 64 * W;                  // (whole waves have an item or none)
+    if (e < 64 * MT * NT) sc[p].load(a, m0 + e / (4 * NT), n0 + 4 * (e % (4 * NT)));
+  }
   i32x4_t acc[MT][NT];
 #pragma unroll
   for (int s = 0; s < MT; ++s)
@@ -185,21 +224,22 @@ __global__ __launch_bounds__(64 * W) void i8_ring_kernel(const I8Args a) {
     if (u + D < n) issue(stage, u + D);
     if (++stage == D) stage = 0;
   }
-  __syncthreads();
-  int* sum = reinterpret_cast<int*>(lds);
-  for (int e = t; e < 16 * MT * LD; e += 64 * W) sum[e] = 0;
-  __syncthreads();
+  // the wave's sums take the place of its ring
+  int* sum = reinterpret_cast<int*>(lds + wave * D * STAGE);
 #pragma unroll
   for (int s = 0; s < MT; ++s)
 #pragma unroll
-    for (int r = 0; r < NT; ++r)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) atomicAdd(&sum[(16 * s + i) * LD + 16 * r + 4 * g + j], acc[s][r][j]);
+    for (int r = 0; r < NT; ++r) *reinterpret_cast<i32x4_t*>(&sum[(16 * s + i) * LD + 16 * r + 4 * g]) = acc[s][r];
   __syncthreads();
-  for (int e = t; e < 16 * MT * 4 * NT; e += 64 * W) {
-    const int m = e / (4 * NT), c = e % (4 * NT);
-    if (m0 + m < a.M && n0 + 4 * c < a.N)
-      i8_store4(a, m0 + m, n0 + 4 * c, *reinterpret_cast<const i32x4_t*>(&sum[m * LD + 4 * c]), a.sx[m0 + m]);
+#pragma unroll
+  for (int p = 0; p < ITEMS; ++p) {
+    const int e = t + p * 64 * W, m = e / (4 * NT), c = e % (4 * NT);
+    if (e < 64 * MT * NT && m0 + m < a.M && n0 + 4 * c < a.N) {
+      i32x4_t v = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < W; ++q) v += *reinterpret_cast<const i32x4_t*>(lds + q * D * STAGE + (m * LD + 4 * c) * 4);
+      i8_store4(a, m0 + m, n0 + 4 * c, v, sc[p]);
+    }
   }
 }
 
@@ -260,6 +300,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
   const int slot = lane & 7, lr = lane >> 3;
   const uint32_t lbase = i8_lds(lds);
   int lt = 0, lk = 0, lm0, ln0;
+  int pm0 = 0, pn0 = 0, pm1 = 0, pn1 = 0;          // places of an even and of an odd tile
   uint32_t off[NL];
   const int8_t *xb, *wb;
   const auto row_of = [&](int j) __attribute__((always_inline)) {   // LDS row of load j in its operand's half
@@ -267,6 +308,13 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
   };
   const auto next_tile = [&]() __attribute__((always_inline)) {
     i8_place(a, first + lt * stride, BM, BN, lm0, ln0);
+    if (lt & 1) {
+      pm1 = lm0;
+      pn1 = ln0;
+    } else {
+      pm0 = lm0;
+      pn0 = ln0;
+    }
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int r = row_of(j), c = slot ^ ((r >> 1) & 7);
@@ -385,8 +433,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
   };
   const auto finish = [&]() __attribute__((always_inline)) {
     asm volatile("" ::: "memory");                 // the stores come after the loads of this k-tile
-    int em0, en0;
-    i8_place(a, first + et * stride, BM, BN, em0, en0);
+    const int em0 = et & 1 ? pm1 : pm0, en0 = et & 1 ? pn1 : pn0;
     const float* sc = reinterpret_cast<const float*>(lds + S * C::STAGE + (et & 1) * C::SC);
     const int nl = wn * 32 * NI + NI * i, n = en0 + nl;
     float sw[NI], bs[NI];
@@ -464,25 +511,23 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void i8_tile_kernel(const I8Args a
 }
 
 // ------------------------------------------------------------------ choice
-// The time of a form is close to a + n (b + d k) us: n tiles fall to the
-// busiest CU, each with k = ceil(K / 128) k-tiles.  a, b and d are fitted to
-// 150 sizes (1 to 4096 rows by [2560 x 640], [640 x 2560], [64 x 2560],
-// [1280 x 2560], [16384 x 2560], [2560 x 6144], [4096 x 4096], [512 x 10240],
-// [10000 x 1280], [18000 x 256], weights from HBM); the form with the least
-// estimate takes 0.9% more than the fastest on average (geometric), 21% at
-// most.  Leaving any one form out costs 1.5 to 2.9%, up to 41% on one size,
-// but for 64 x 64 tiles in the ring (no loss on average, 10% on one size),
-// which are left out.
 constexpr int64_t kI8MaxStride = (1 << 24) - 16;   // 256 rows within 32-bit offsets
 
+// The time of a form is close to a + n (b + d k) us: n tiles fall to the
+// busiest CU, each with k = ceil(K / 128) k-tiles.  a, b and d are fitted to
+// 490 sizes (1 to 4096 rows, 16 to 18000 columns, K from 64 to 10240, most of
+// them drawn evenly over their logarithms; weights from HBM), and the form with
+// the least estimate is taken: 0.7% more than the fastest on average there, 1.4%
+// at 120 sizes that the fit has not seen, 22% at most.  Leaving any one form out
+// costs 0.1 to 4.2% on average and 22 to 200% on one size.
 struct I8Form { int bm, bn, slots, ring, stages; float a, b, d; };
 constexpr I8Form kI8Forms[] = {
-    {16, 16, 2, 1, 2, 1.68f, 0.61f, 0.042f},   {16, 32, 2, 1, 3, 1.73f, 0.66f, 0.066f},
-    {16, 64, 2, 1, 2, 1.79f, 0.81f, 0.108f},   {32, 32, 2, 1, 2, 1.62f, 0.82f, 0.087f},
-    {32, 64, 1, 1, 2, 0.55f, 2.54f, 0.139f},   {64, 64, 2, 0, 4, 2.75f, 0.69f, 0.223f},
-    {64, 128, 2, 0, 3, 3.09f, 1.04f, 0.336f},  {128, 128, 1, 0, 4, 0.96f, 3.15f, 0.453f},
-    {128, 128, 2, 0, 2, 3.15f, 1.38f, 0.564f}, {256, 128, 1, 0, 3, 0.34f, 5.29f, 0.710f},
-    {256, 256, 1, 0, 2, 1.02f, 7.51f, 1.270f}};
+    {16, 16, 2, 1, 2, 2.14f, 0.53f, 0.028f}, {16, 32, 2, 1, 3, 2.13f, 0.57f, 0.061f},
+    {16, 64, 2, 1, 2, 2.26f, 0.62f, 0.111f}, {32, 32, 2, 1, 2, 2.18f, 0.59f, 0.076f},
+    {32, 64, 1, 1, 2, 1.32f, 2.20f, 0.144f}, {64, 64, 2, 0, 4, 2.67f, 0.77f, 0.276f},
+    {64, 128, 2, 0, 3, 2.93f, 1.12f, 0.312f}, {128, 128, 1, 0, 4, 0.89f, 2.80f, 0.519f},
+    {128, 128, 2, 0, 2, 3.00f, 1.72f, 0.583f}, {256, 128, 1, 0, 3, 2.43f, 4.24f, 0.855f},
+    {256, 256, 1, 0, 2, 5.83f, 5.42f, 1.341f}};
 
 template <int BM, int BN, int WM, int WN, int S>
 static void launch_i8_tile(dim3 grid, const I8Args& a, hipStream_t st) {
