@@ -480,6 +480,40 @@ def test_side_stream(F):
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_outputs_are_released(F):
+    """Outputs are held by their callers alone, after calls that raise too."""
+    import sys
+    x, r = rows(1, 64, 2571, "bf16").cuda(), rows(2, 64, 2571, "bf16").cuda()
+    w = torch.ones(2571).bfloat16().cuda()
+
+    def once():
+        q, s, h, y = F.rms_norm_q8(x, w, residual=r, normed=True)
+        z = F.w8a8_linear(q, s, q, s)
+        g = F.silu_mul_q8(x, r, "e4m3")
+        for bad in (lambda: F.rms_norm_q8(x, w, residual=r, eps=-1.0), lambda: F.w8a8_linear(q, s, q, s[:1])):
+            with pytest.raises(ValueError):
+                bad()
+        return [sys.getrefcount(t) for t in (q, s, h, y, z, *g)]
+    counts = once()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(50):
+        assert once() == counts
+    assert max(counts) <= 4                          # the variable, the list's or tuple's entry, the argument
+    assert torch.cuda.memory_allocated() == before
+
+
+def test_norm_into_its_own_rows(F):
+    """The next residual may be written over the residual, or over x."""
+    for h in (17, 512, 2571, 9001):
+        x, r, w = rows(3, 70, h, "bf16").cuda(), rows(4, 70, h, "bf16").cuda(), torch.ones(h).bfloat16().cuda()
+        want = F.rms_norm_q8(x, w, residual=r)
+        for over in (0, 1):
+            a, b = x.clone(), r.clone()
+            got = F.rms_norm_q8(a, w, residual=b, residual_out=b if over else a)
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_refusals_on_device(F):
     x = torch.ones((2, 64), device="cuda").bfloat16()
     w = torch.ones(64, device="cuda").bfloat16()
@@ -494,6 +528,12 @@ def test_refusals_on_device(F):
             (lambda: F.rms_norm_q8(x, w, eps=-1.0), ValueError),
             (lambda: F.rms_norm_q8(x, w, eps=float("nan")), ValueError),
             (lambda: F.rms_norm_q8(x, w, fmt="int4"), ValueError),
+            (lambda: F.rms_norm_q8(x, w, fmt=1), ValueError),
+            (lambda: F.rms_norm_q8(x, w, eps="a"), TypeError),
+            (lambda: F.rms_norm_q8(x, w, w_offset=None), TypeError),
+            (lambda: F.rms_norm_q8(x, w, residual=x, residual_out=x.cpu()), RuntimeError),
+            (lambda: F.silu_mul_q8(x, x.cpu()), RuntimeError),
+            (lambda: F.w8a8_linear(q, s, q, s, out_dtype="bf16"), TypeError),
             (lambda: F.rms_norm_q8(x.double(), w), TypeError),
             (lambda: F.rms_norm_q8(x[0], w), ValueError),
             (lambda: F.rms_norm_q8(x, w.cpu()), RuntimeError),

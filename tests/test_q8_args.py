@@ -71,6 +71,19 @@ def test_cpu_tensors_raise():
             call()
 
 
+def test_wrong_types_raise():
+    import _fp4x
+    import fp4x_kernels as F
+    x = torch.ones((2, 64)).bfloat16()
+    for call in (lambda: F.quantize_q8("x"), lambda: F.quantize_q8(None), lambda: F.silu_mul_q8([1.0]),
+                 lambda: F.rms_norm_q8(x, None), lambda: F.w8a8_linear(x, x, x, 3)):
+        with pytest.raises(TypeError):
+            call()
+    for name, n in (("rms_norm_q8", 8), ("silu_mul_q8", 3), ("quantize_q8", 2), ("w8a8_linear", 6)):
+        with pytest.raises(TypeError):
+            getattr(_fp4x.host(), name)(*[x] * (n - 1))
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3", "mx8"])
 def test_oracle_against_torch(fmt):
     """The oracle's codes are the nearest ones: no other code of the format is closer to v / s."""
