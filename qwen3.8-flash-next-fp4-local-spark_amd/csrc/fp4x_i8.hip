@@ -543,8 +543,10 @@ static void launch_i8(I8Args a, hipStream_t st) {
   a.nt = (a.N + f.bn - 1) / f.bn;
   a.gm = f.ring ? a.mt : 4;                        // 4 x 8 tiles of 256 x 256 are what the CUs of an XCD work on
   const int tiles = a.mt * a.nt, slots = f.slots * device_cus();
-  // several tiles per workgroup: the loads run at most one tile ahead
-  const dim3 grid(!f.ring && tiles > slots && (a.K + 127) / 128 >= f.stages ? slots : tiles);
+  // Several tiles per workgroup only where a tile has more k-tiles than the ring has stages: the scales of tile t + 2
+  // take the place of tile t's when the last load of tile t + 1 is out, which is then behind a barrier that every wave
+  // comes to after its part of tile t's epilogue.
+  const dim3 grid(!f.ring && tiles > slots && (a.K + 127) / 128 > f.stages ? slots : tiles);
   if constexpr (F == 0) hipLaunchKernelGGL((i8_ring_kernel<1, 1, 8, 2>), grid, dim3(512), 0, st, a);
   else if constexpr (F == 1) hipLaunchKernelGGL((i8_ring_kernel<1, 2, 4, 3>), grid, dim3(256), 0, st, a);
   else if constexpr (F == 2) hipLaunchKernelGGL((i8_ring_kernel<1, 4, 4, 2>), grid, dim3(256), 0, st, a);

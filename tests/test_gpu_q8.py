@@ -328,6 +328,19 @@ def test_linear_forms(F, m, n, k):
     same(y[torch.from_numpy(rows).cuda()], rounder(out)(want), (m, n, k, out))
 
 
+# many tiles of as many k-tiles as a form has stages, one more and one less
+@pytest.mark.parametrize("m,n", [(2851, 18470), (1100, 16390), (2000, 9000), (600, 20000), (4100, 6000), (70, 60000)])
+@pytest.mark.parametrize("k", [199, 256, 300, 384, 400, 512, 520, 640])
+def test_linear_short_sums_of_many_tiles(F, m, n, k):
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    xq, wq = (torch.randint(-128, 128, (r, (k + 15) // 16 * 16), generator=g, device="cuda", dtype=torch.int8)[:, :k]
+              for r in (m, n))
+    xs, ws, b = (0.5 + torch.rand(r, generator=g, device="cuda") for r in (m, n, n))
+    want = ((xq.float() @ wq.float().t()) * xs[:, None]) * ws + b   # sums below 2^24 are exact in fp32
+    for _ in range(3):
+        assert torch.equal(F.w8a8_linear(xq, xs, wq, ws, b, torch.float32), want)
+
+
 def test_linear_forms_are_all_reached(F):
     import _fp4x
     form = _fp4x.lib().fp4x_w8a8_form
