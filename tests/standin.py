@@ -18,6 +18,7 @@ RUNTIME = r"""
 #include <string>
 struct dim3_ { unsigned x, y, z; };
 static std::map<const void*, std::string>& names() { static auto* m = new std::map<const void*, std::string>; return *m; }
+static std::string& grids() { static auto* s = new std::string; return *s; }
 static std::string& log_() { static auto* s = new std::string; return *s; }
 static int last = 0;
 static dim3_ cfg_grid, cfg_block;
@@ -42,12 +43,14 @@ int __hipPushCallConfiguration(dim3_ g, dim3_ b, size_t, void*) { cfg_grid = g; 
 int __hipPopCallConfiguration(dim3_* g, dim3_* b, size_t* s, void** st) {
   *g = cfg_grid; *b = cfg_block; *s = 0; *st = nullptr; return 0;
 }
-int hipLaunchKernel(const void* fn, dim3_, dim3_, void**, size_t, void*) {
+int hipLaunchKernel(const void* fn, dim3_ g, dim3_ b, void**, size_t, void*) {
   log_() += names()[fn] + "\n";
+  grids() += std::to_string(g.x) + " " + std::to_string(b.x) + "\n";
   return 0;
 }
+const char* fp4x_test_grids(void) { return grids().c_str(); }
 const char* fp4x_test_log(void) { return log_().c_str(); }
-void fp4x_test_clear(void) { log_().clear(); }
+void fp4x_test_clear(void) { log_().clear(); grids().clear(); }
 }
 """
 
