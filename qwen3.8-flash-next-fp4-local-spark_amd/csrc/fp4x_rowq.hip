@@ -163,9 +163,13 @@ __device__ __forceinline__ T row_reduce(T v, int L, T* slot, Op op) {
   return v;
 }
 
-// x * sigmoid(x) within about 3 fp32 ulps (expf, v_rcp_f32); 0 below about
-// -87, where the exact value is under 2e-36.
-__device__ __forceinline__ float silu_f32(float x) { return x * __builtin_amdgcn_rcpf(1.0f + expf(-x)); }
+// x * sigmoid(x) from an expf within an ulp and a quotient that is the rounded
+// one below 2^100 (one correction of the reciprocal); 0 below about -87, where
+// the exact value is under 2e-36.
+__device__ __forceinline__ float silu_f32(float x) {
+  const float d = 1.0f + expf(-x), r = __builtin_amdgcn_rcpf(d);
+  return x * (d < 0x1p100f ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : r);
+}
 
 __device__ __forceinline__ uint32_t e4m3x4(const float* f) {
   int d = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
