@@ -269,7 +269,9 @@ int fp4x_quantize_nv4(int src, const void* src_a, const void* src_b, float src_g
  * rms_norm_q8: h = x + res rounded to res_dtype (x itself when res is NULL);
  * v = (h * rs) * (w + w_offset), rs = fp32(1 / sqrt(mean(h^2) + eps)), the mean
  * in fp64.  res and w have x's dtype or are fp32.  res_out (optional, res_dtype)
- * receives h and may be res itself; normed (optional, dtype) receives v. */
+ * receives h; it may be res or x itself (the same rows), or lie between their
+ * rows, but shares no other memory with an input.  normed (optional, dtype)
+ * receives v.  q, s and normed share no memory with anything else. */
 int fp4x_rms_norm_q8(const void* x, int64_t x_stride, int dtype, const void* res, int64_t res_stride, int res_dtype,
                      const void* w, int w_dtype, float w_offset, double eps, int M, int H, int fmt, void* q,
                      int64_t q_stride, void* s, void* res_out, int64_t res_out_stride, void* normed,

@@ -384,6 +384,34 @@ static int row_fail(const char* what, const char* why) {
 static bool el_aligned(const void* p, int dt) {
   return (reinterpret_cast<uintptr_t>(p) & (dt == DT_F32 ? 3 : 1)) == 0;
 }
+// M rows of n bytes, `step` bytes apart (0: one row read M times).
+struct RowSpan {
+  uintptr_t at;
+  int64_t step, n, M;
+  RowSpan(const void* p, int dt, int64_t stride, int H, int M_)
+      : at(reinterpret_cast<uintptr_t>(p)), step(M_ > 1 ? stride * (dt == DT_F32 ? 4 : 2) : 0),
+        n((int64_t)H * (dt == DT_F32 ? 4 : 2)), M(step ? M_ : 1) {}
+  uintptr_t end() const { return at + (M - 1) * step + n; }
+};
+static bool same_rows(const RowSpan& a, const RowSpan& b) {
+  return a.at == b.at && a.n == b.n && a.M == b.M && a.step == b.step;
+}
+// Whether a row of b shares a byte with a row of a, whose own rows do not overlap.
+static bool meet(const RowSpan& a, const RowSpan& b) {
+  if (a.end() <= b.at || b.end() <= a.at) return false;
+  if (a.M > 1 && a.step == b.step) {               // every period is alike
+    const RowSpan &p = a.at <= b.at ? a : b, &q = a.at <= b.at ? b : a;
+    const int64_t d = (int64_t)(q.at - p.at) % a.step;
+    return d < p.n || d + q.n > a.step;
+  }
+  for (int64_t i = 0; i < b.M; ++i) {
+    const uintptr_t from = b.at + i * b.step, to = from + b.n;
+    if (to <= a.at) continue;
+    const int64_t j = a.M > 1 ? std::min<int64_t>(a.M - 1, (int64_t)(to - 1 - a.at) / a.step) : 0;
+    if (a.at + j * a.step + a.n > from) return true;   // the last row of a that begins before b's row i ends
+  }
+  return false;
+}
 static bool known_dt(int dt) { return dt == DT_BF16 || dt == DT_F32 || dt == DT_F16; }
 
 // What the three entry points share; 0 rows: nothing else is looked at.
@@ -424,6 +452,13 @@ int fp4x_rms_norm_q8(const void* x, int64_t x_stride, int dtype, const void* res
   if (res_out && !res) return row_fail(what, "a residual output needs a residual");
   if (res_stride < 0 || (M > 1 && ((res_out && res_out_stride < H) || (normed && normed_stride < H))))
     return row_fail(what, "output rows overlap, or a row stride is negative");
+  if (res_out) {                                   // workgroups read and write rows in no order: each its own only
+    const RowSpan out(res_out, res_dtype, res_out_stride, H, M);
+    for (const RowSpan& in : {RowSpan(x, dtype, x_stride, H, M), RowSpan(res, res_dtype, res_stride, H, M)})
+      if (!same_rows(out, in) && meet(out, in))
+        return row_fail(what, "the residual output overlaps an input whose rows it does not replace one for one");
+    if (meet(out, RowSpan(w, w_dtype, 0, H, 1))) return row_fail(what, "the residual output overlaps the norm weight");
+  }
   hipStream_t st = (hipStream_t)stream;
   const bool r32 = res_dtype == DT_F32, w32 = w_dtype == DT_F32;
   if (dtype == DT_F32) return launch_row_q8<ROW_NORM, DT_F32, DT_F32, DT_F32>(a, st);

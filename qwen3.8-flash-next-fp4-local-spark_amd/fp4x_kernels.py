@@ -207,7 +207,8 @@ def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=
     h = x + residual (rounded to the residual's type), v = h / sqrt(mean(h^2)
     + eps) * (w + w_offset).  Returns (q, s) of v in `fmt`; with a residual
     also h, the next residual (written to residual_out if given, which may be
-    the residual itself); with normed=True also v in x's type.
+    the residual or x itself but shares no other memory with an input); with
+    normed=True also v in x's type.
 
     fmt "int8": int8 codes and fp32 scales [M] (w8a8_linear takes them);
     "e4m3": the same with float8_e4m3fn codes; "mx8": MXFP8, float8_e4m3fn
