@@ -214,7 +214,8 @@ def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=
     "e4m3": the same with float8_e4m3fn codes; "mx8": MXFP8, float8_e4m3fn
     codes and uint8 e8m0 scales [M, H/32].  A row (mx8: a block) with an
     infinity or a NaN gets the scale NaN.  x is bf16, fp16 or fp32; residual
-    and w have its type or are fp32.  1 <= H <= 32768."""
+    and w have its type or are fp32.  1 <= H <= 32768.  q and s of up to 1 MiB
+    together share one storage."""
     return _L.host().rms_norm_q8(x, w, eps, residual, fmt, w_offset, normed, residual_out)
 
 

@@ -1,0 +1,56 @@
+"""The 8-bit activation path on the GPU, at its edges: what outputs keep alive,
+rows past the grid, code rows that end their storage, and whole k-tiles in every
+form of the product.  Results equal the definition bit for bit."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def F(gpu):
+    import fp4x_kernels
+    return fp4x_kernels
+
+
+def pairs(F, fmt, m, h):
+    x = torch.randn((m, h), generator=torch.Generator("cuda").manual_seed(m), device="cuda").bfloat16()
+    w = torch.ones(h, device="cuda").bfloat16()
+    yield lambda: F.quantize_q8(x, fmt)
+    yield lambda: F.silu_mul_q8(x, x, fmt)
+    yield lambda: F.rms_norm_q8(x, w, fmt=fmt)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "mx8"])
+def test_codes_and_scales_are_released_alone(F, fmt):
+    """Above 1 MiB neither of them holds the other's memory; below, no more than that."""
+    for m, h in ((4096, 640), (1640, 640), (1740, 608), (1030, 32768)):
+        for make in pairs(F, fmt, m, h):
+            q, s = make()
+            per = 4 * m if fmt != "mx8" else m * h // 32
+            assert q.shape == (m, h) and q.stride() == (h, 1) and s.numel() * s.element_size() == per
+            torch.cuda.synchronize()
+            assert q.untyped_storage().nbytes() == m * h and s.untyped_storage().nbytes() == per
+            before = torch.cuda.memory_allocated()
+            del q
+            assert before - torch.cuda.memory_allocated() >= m * h
+    for m, h in ((3, 2560), (512, 640), (1, 32)):
+        for make in pairs(F, fmt, m, h):
+            q, s = make()
+            assert max(t.untyped_storage().nbytes() for t in (q, s)) <= 1 << 20
+
+
+def test_padded_codes_of_many_rows(F):
+    x = torch.randn((900, 2571), generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    q, s = F.quantize_q8(x)
+    assert q.stride() == (2576, 1) and q.untyped_storage().nbytes() == 900 * 2576 and q.data_ptr() % 16 == 0
+    amax = x.abs().amax(-1)
+    want = amax / torch.full_like(amax, 127.0)
+    assert torch.equal(s, want) and torch.equal(q, (x / want[:, None]).round().to(torch.int8))
+    q1, s1 = F.quantize_q8(x[:100])                  # one allocation
+    assert torch.equal(q1, q[:100]) and torch.equal(s1, s[:100])
+    w = torch.randn((64, 2571), generator=torch.Generator("cuda").manual_seed(2), device="cuda")
+    qw, sw = F.quantize_q8(w)
+    acc = (q.double() @ qw.double().t()).float()
+    assert torch.equal(F.w8a8_linear(q, s, qw, sw, out_dtype=torch.float32), acc * s[:, None] * sw)
