@@ -190,6 +190,7 @@ __global__ __launch_bounds__(64 * W) void i8_ring_kernel(const I8Args a) {
     const int e = t + p * 64 * W;                  // (whole waves have an item or none)
     if (e < 64 * MT * NT) sc[p].load(a, m0 + e / (4 * NT), n0 + 4 * (e % (4 * NT)));
   }
+  asm volatile("" ::: "memory");                   // not behind the units' loads, whose waits count what is newer
   i32x4_t acc[MT][NT];
 #pragma unroll
   for (int s = 0; s < MT; ++s)
