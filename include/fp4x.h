@@ -276,7 +276,8 @@ int fp4x_rms_norm_q8(const void* x, int64_t x_stride, int dtype, const void* res
                      const void* w, int w_dtype, float w_offset, double eps, int M, int H, int fmt, void* q,
                      int64_t q_stride, void* s, void* res_out, int64_t res_out_stride, void* normed,
                      int64_t normed_stride, void* stream);
-/* v = silu(gate) * up, within a few fp32 ulps before the quantization. */
+/* v = silu(gate) * up, within a few fp32 ulps before the quantization; gates
+ * below about -87, where silu is under 2e-36 in magnitude, may count as 0. */
 int fp4x_silu_mul_q8(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int dtype, int M, int F,
                      int fmt, void* q, int64_t q_stride, void* s, void* stream);
 /* v = x (activations per token, or a weight per output channel). */

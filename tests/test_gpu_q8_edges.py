@@ -5,6 +5,9 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import q8 as o8
+from oracle.formats import e4m3_decode
+
 pytestmark = pytest.mark.gpu
 
 
@@ -54,3 +57,23 @@ def test_padded_codes_of_many_rows(F):
     qw, sw = F.quantize_q8(w)
     acc = (q.double() @ qw.double().t()).float()
     assert torch.equal(F.w8a8_linear(q, s, qw, sw, out_dtype=torch.float32), acc * s[:, None] * sw)
+
+
+# silu(g) * u above -69 in steps of 2^-24: expf within an ulp (2), 1 + t (1), the rounded quotient (1) and two products (1
+# each): v is within 6.  The scale adds its division: 7.  A code's quotient v / s adds both and its own division: 14.
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_silu_roundings(F, fmt, dt):
+    step = 2.0 ** -24
+    for m, f, spread in ((900, 1030, 2.0), (300, 4100, 8.0)):
+        g = torch.Generator("cuda").manual_seed(m)
+        gate, up = ((spread * torch.randn((m, f), generator=g, device="cuda")).clamp(-68, 68).to(dt) for _ in range(2))
+        q, s = F.silu_mul_q8(gate, up, fmt)
+        v = o8.silu_mul(gate.float().cpu().numpy(), up.float().cpu().numpy())
+        s64 = np.abs(v).max(-1) / (127 if fmt == "int8" else 448)
+        s = s.cpu().numpy().astype(np.float64)
+        assert (np.abs(s - s64) <= 7 * step * s64).all()
+        y = v / s[:, None]
+        got = q.cpu().numpy().astype(np.float64) if fmt == "int8" else e4m3_decode(q.view(torch.uint8).cpu().numpy()).astype(np.float64)
+        half = 0.5 if fmt == "int8" else np.maximum(np.abs(y) * 2.0 ** -4, 2.0 ** -10)
+        assert (np.abs(got - y) <= half + 14 * step * np.abs(y)).all()
