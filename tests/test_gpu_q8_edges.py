@@ -77,3 +77,31 @@ def test_silu_roundings(F, fmt, dt):
         got = q.cpu().numpy().astype(np.float64) if fmt == "int8" else e4m3_decode(q.view(torch.uint8).cpu().numpy()).astype(np.float64)
         half = 0.5 if fmt == "int8" else np.maximum(np.abs(y) * 2.0 ** -4, 2.0 ** -10)
         assert (np.abs(got - y) <= half + 14 * step * np.abs(y)).all()
+
+
+# every form with a K of whole k-tiles, with one and with several tiles per workgroup (tests/test_q8_routes_whole.py asserts
+# that no kind is missing); full tiles and tiles that end at M or N
+WHOLE = [(2, 48, 128), (1, 2560, 640), (1, 5449, 128), (3, 7000, 256), (16, 9779, 128), (9, 16384, 2560), (48, 520, 512), (5903, 2, 128),
+         (34, 9820, 2688), (40, 9820, 2560), (34, 9820, 128), (8203, 35, 128), (100, 8200, 256), (18, 28777, 256), (96, 9332, 1280),
+         (137, 23097, 512), (65, 35114, 640), (67, 38063, 640), (300, 5200, 1024), (35, 17360, 128), (250, 13310, 2560),
+         (344, 16725, 640), (286, 20549, 640), (556, 12116, 1280), (325, 22293, 128), (194, 36551, 128), (476, 20646, 384),
+         (4824, 2078, 384), (783, 12600, 640), (413, 13957, 128), (1100, 8192, 1024), (4121, 1424, 128), (652, 29929, 512),
+         (2487, 6505, 640), (1100, 16384, 2560), (1536, 13312, 2560), (7510, 2118, 512), (1364, 9261, 256), (6621, 1864, 256),
+         (668, 34914, 384), (3897, 6505, 384), (2048, 16384, 640), (1111, 16390, 1024), (61, 5250, 2816), (778, 334, 2688)]
+
+
+# kinds with a K inside a k-tile that sizes of ragged M and N seldom take
+RAGGED = [(258, 20721, 627), (340, 18892, 540), (695, 33195, 326), (1535, 17023, 295)]
+
+
+@pytest.mark.parametrize("m,n,k", WHOLE + RAGGED)
+def test_products_of_every_kind(F, m, n, k):
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    xq, wq = (torch.randint(-128, 128, (r, k + 15 & -16), generator=g, device="cuda", dtype=torch.int8)[:, :k] for r in (m, n))
+    xs, ws, b = (0.5 + torch.rand(r, generator=g, device="cuda") for r in (m, n, n))
+    acc = (xq.double() @ wq.double().t()).float()    # the exact sum, rounded once
+    y = (acc * xs[:, None]) * ws
+    for _ in range(3):
+        assert torch.equal(F.w8a8_linear(xq, xs, wq, ws, b, torch.float32), y + b)
+    assert torch.equal(F.w8a8_linear(xq, xs, wq, ws), y.bfloat16())
+    assert torch.equal(F.w8a8_linear(xq, xs, wq, ws, out_dtype=torch.float16).view(torch.int16), y.half().view(torch.int16))
