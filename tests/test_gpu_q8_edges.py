@@ -105,3 +105,40 @@ def test_products_of_every_kind(F, m, n, k):
         assert torch.equal(F.w8a8_linear(xq, xs, wq, ws, b, torch.float32), y + b)
     assert torch.equal(F.w8a8_linear(xq, xs, wq, ws), y.bfloat16())
     assert torch.equal(F.w8a8_linear(xq, xs, wq, ws, out_dtype=torch.float16).view(torch.int16), y.half().view(torch.int16))
+
+
+# more rows than a grid of 2^20 workgroups takes at once: rows of a wave's part, of a wave and of several waves (2, 3 and 4
+# chunks per lane), each a window of one vector, eight values on from the row before
+CAP = 1 << 20
+PAST = [(64 * CAP + 5, 16), (4 * CAP + 5, 264), (CAP + 3, 1032), (CAP + 1031, 1056), (CAP + 3, 4104), (CAP + 3, 24584)]
+
+
+@pytest.mark.parametrize("m,h", PAST)
+def test_rows_past_the_grid(F, m, h):
+    g = torch.Generator("cuda").manual_seed(h)
+
+    def windows():
+        v = torch.randn(8 * m + h, generator=g, device="cuda").bfloat16()
+        return v.as_strided((m, h), (8, 1))
+    x, r = windows(), windows()
+    w = (1 + 0.2 * torch.randn(h, generator=g, device="cuda")).bfloat16()
+    at = torch.cat([torch.arange(40), torch.arange(m - 40, m), torch.linspace(0, m - 1, 40).long()]).cuda()
+    cut = m // 2                                     # a call of half as many rows takes one pass
+
+    def both(call, oracle):
+        whole = call(slice(None))
+        for part in (slice(0, cut), slice(cut, None)):
+            for a, b in zip(whole, call(part)):
+                assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8))
+                           for p, q in zip(a[part].split(1 << 20), b.split(1 << 20)))
+        for a, b in zip(whole, oracle):
+            a = a[at].cpu()
+            a = a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a.float() if a.dtype == torch.bfloat16 else a
+            assert np.array_equal(a.numpy(), b)
+    xs, rs = x[at].float().cpu().numpy(), r[at].float().cpu().numpy()
+    fmt = "mx8" if h % 32 == 0 else "int8"
+    both(lambda p: F.quantize_q8(x[p], fmt), o8.quantize(xs, fmt))
+    if h > 8192:                                     # (26 GB of codes are enough)
+        return
+    v, n = o8.rms_norm(xs, w.float().cpu().numpy(), 1e-6, rs, lambda a: torch.from_numpy(a).bfloat16().float().numpy())
+    both(lambda p: F.rms_norm_q8(x[p], w, residual=r[p], fmt=fmt), (*o8.quantize(v, fmt), n))

@@ -1,14 +1,15 @@
 """The sizes that the GPU tests run cover every kind of launch of
 w8a8_linear, without a GPU (tests/standin.py, 256 CUs): each form, with a K of
 whole k-tiles and one that ends inside a k-tile, with one and with several
-tiles per workgroup, as far as the choice of a form leads there at all."""
+tiles per workgroup, as far as the choice of a form leads there at all; and the row kernels past their
+largest grid."""
 import json
 
 import pytest
 
 import standin
 from test_gpu_q8 import FORM_KS, FORMS
-from test_gpu_q8_edges import RAGGED, WHOLE
+from test_gpu_q8_edges import CAP, PAST, RAGGED, WHOLE
 
 
 @pytest.fixture(scope="module")
@@ -53,3 +54,18 @@ print(json.dumps(sorted(out)))
     assert drawn <= ran, sorted(drawn - ran)
     # what the choice does not lead to: several tiles of 64 x 64 per workgroup
     assert not any(f == 5 and several for f, _, several in drawn | ran)
+
+
+def test_rows_past_the_grid(route):
+    """Sizes that take a workgroup through its row loop more than once, with rows of part of a wave, of one wave and of
+    several, and each number of chunks per lane that so many rows lead to."""
+    got = route(KIND + f"""
+out = []
+for M, H in {PAST!r}:
+    rc, names = launched(L.fp4x_quantize_q8, P, 8, B.DT_BF16, M, H, 0, P, H + 15 & -16, P, None)
+    assert rc == B.OK and len(names) == 1
+    out.append([*map(int, rt.fp4x_test_grids().split()), int(re.findall(r"Li(\\d+)E", names[0])[-1])])
+print(json.dumps(out))
+""")
+    assert all(grid == CAP for grid, _, _ in got)
+    assert [(block, chunks) for _, block, chunks in got] == [(256, 1), (256, 2), (128, 2), (128, 2), (192, 3), (832, 4)]
