@@ -142,3 +142,31 @@ def test_rows_past_the_grid(F, m, h):
         return
     v, n = o8.rms_norm(xs, w.float().cpu().numpy(), 1e-6, rs, lambda a: torch.from_numpy(a).bfloat16().float().numpy())
     both(lambda p: F.rms_norm_q8(x[p], w, residual=r[p], fmt=fmt), (*o8.quantize(v, fmt), n))
+
+
+def copies(call):
+    """A call's result and how many allocations it makes."""
+    call()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    y = call()
+    return y, torch.cuda.memory_stats()["allocation.all.allocated"] - before
+
+
+def test_code_rows_that_end_their_storage(F):
+    """The last row may end inside a chunk of 16 bytes only where the storage goes on to its end; otherwise it is copied."""
+    k = 9
+    w, one = torch.ones((5, k), dtype=torch.int8, device="cuda"), torch.ones(5, device="cuda")
+    wq = torch.zeros((5, 16), dtype=torch.int8, device="cuda")[:, :k]
+    wq.copy_(w)
+    xs = 1 + torch.arange(20, device="cuda").float()
+    for end, allocations in ((16 * 19 + k, 2), (16 * 19 + 15, 2), (16 * 20, 1)):   # the output, and a copy
+        flat = torch.full((end,), 7, dtype=torch.int8, device="cuda")
+        assert flat.untyped_storage().nbytes() == end and flat.data_ptr() % 16 == 0
+        x = flat.as_strided((20, k), (16, 1))
+        y, n = copies(lambda: F.w8a8_linear(x, xs, wq, one, out_dtype=torch.float32))
+        assert n == allocations and bool((y == (7 * k * xs)[:, None]).all())
+        y, n = copies(lambda: F.w8a8_linear(wq, one, x, xs, out_dtype=torch.float32))   # as weights
+        assert n == allocations and bool((y == (7 * k * xs)[None]).all())
+    flat = torch.full((16 * 19 + k + 32,), 7, dtype=torch.int8, device="cuda")
+    x = flat[32:].as_strided((20, k), (16, 1), 32)   # the same rows further on
+    assert copies(lambda: F.w8a8_linear(x, xs, wq, one))[1] == 2
