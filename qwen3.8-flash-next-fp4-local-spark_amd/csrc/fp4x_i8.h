@@ -141,8 +141,8 @@ __device__ __forceinline__ void i8_store4(const I8Args& a, int64_t m, int n, i32
 //
 // What bounds it: the bytes a CU can have on their way.  The same split with
 // loads into registers (16 rows x 64 bytes a load, in the layout that the MFMA
-// takes) takes 14.3 us at 16 x [16384 x 2560] and 13.1 at 64 x [2560 x 6144];
-// this takes 9.8 and 7.1 (weights from HBM).  Scales that are loaded after the
+// takes) took 14.3 us at 16 x [16384 x 2560] and 13.1 at 64 x [2560 x 6144];
+// this takes 8.5 and 7.1 (weights from HBM).  Scales that are loaded after the
 // sums, and sums through atomics on a cleared block of LDS, took 0.6 us more.
 template <int MT, int NT, int W, int D>
 __global__ __launch_bounds__(64 * W) void i8_ring_kernel(const I8Args a) {
@@ -263,16 +263,17 @@ __global__ __launch_bounds__(64 * W) void i8_ring_kernel(const I8Args a) {
 // 64 rows at once, as 16 columns of a row per lane would give, took 13 us more
 // of 4096 x [16384 x 2560]).
 //
-// What bounds it at 4096 x [16384 x 2560] (256 x 256 tiles): 151 us in a long
-// row of calls, 2.3 POP/s.  In copies that leave parts out the MFMAs alone take
-// 100, with LDS reads 116, with the loads too 134, with the conversion 139, with
-// the stores 147.  In cycles the parts overlap (12% between the first and the
-// last), but the clock falls from 2.2 to 1.8 GHz as they add up: the power
-// limit.  Consecutive MFMAs keep one operand for that reason.  A 4-wave form
-// (128 x 128 per wave) takes 174 and more, 16 x 16 x 64 MFMAs 166, k-tiles of 64
-// in four stages 147 (all without stores), where this takes 138; 16 waves take
-// as long.  A K that ends inside a k-tile is code of its own (TAIL): the test for
-// it in every step took 9 us more.
+// What bounds it at 4096 x [16384 x 2560] (256 x 256 tiles): 159 to 181 us among
+// other work (2.2 to 1.9 POP/s), 151 (2.3) in a long row of the same call.  In
+// copies that leave parts out, timed in such rows, the MFMAs alone take 100, with
+// LDS reads 116, with the loads too 134, with the conversion 139, with the stores
+// 147.  In cycles the parts overlap (12% between the first and the last), but the
+// clock falls from 2.2 to 1.8 GHz as they add up: the power limit.  Consecutive
+// MFMAs keep one operand for that reason.  A 4-wave form (128 x 128 per wave)
+// takes 174 and more, 16 x 16 x 64 MFMAs 166, k-tiles of 64 in four stages 147
+// (all without stores), where this takes 138; 16 waves take as long.  A K that
+// ends inside a k-tile is code of its own (TAIL): the test for it in every step
+// took 9 us more.
 template <int BM, int BN, int WM, int WN, int S>
 struct I8Tile {
   static constexpr int W = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;

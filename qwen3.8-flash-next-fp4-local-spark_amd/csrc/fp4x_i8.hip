@@ -12,13 +12,16 @@ int device_cus();
 // ------------------------------------------------------------------ choice
 constexpr int64_t kI8MaxStride = (1 << 24) - 16;   // 256 rows within 32-bit offsets
 
-// The time of a form is close to a + n (b + d k) us: n tiles fall to the
-// busiest CU, each with k = ceil(K / 128) k-tiles.  a, b and d are fitted to
-// 490 sizes (1 to 4096 rows, 16 to 18000 columns, K from 64 to 10240, most of
-// them drawn evenly over their logarithms; weights from HBM), and the form with
-// the least estimate is taken: 0.7% more than the fastest on average there, 1.4%
-// at 120 sizes that the fit has not seen, 22% at most.  Leaving any one form out
-// costs 0.1 to 4.2% on average and 22 to 200% on one size.
+// Forms are ranked by a + n (b + d k) us: n tiles fall to the busiest CU, each
+// with k = ceil(K / 128) k-tiles.  a, b and d are fitted to 490 sizes (1 to 4096
+// rows, 16 to 18000 columns, K from 64 to 10240, most of them drawn evenly over
+// their logarithms; weights from HBM), and the form with the least estimate is
+// taken.  Over the 608 sizes on record it takes 0.7% more than the fastest on
+// average at 489 of the fit and 1.6% at 119 that the fit has not seen, 24% at
+// most.  Leaving any one form out costs 0.1 to 4.5% on average and 19 to 104% at
+// one size.  As a time the estimate of the chosen form is good to -6 .. +37% at
+// 90% of the sizes, and up to 2.4 times too low where few rows wait for the
+// weights' bytes, which it does not count.
 struct I8Form { int bm, bn, slots, ring, stages; float a, b, d; };
 constexpr I8Form kI8Forms[] = {
     {16, 16, 2, 1, 2, 2.14f, 0.53f, 0.028f}, {16, 32, 2, 1, 3, 2.13f, 0.57f, 0.061f},

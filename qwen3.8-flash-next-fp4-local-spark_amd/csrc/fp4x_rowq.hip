@@ -12,9 +12,9 @@
 // The norm: h = x + r in fp32, rounded once to r's type and written back as
 // the residual; v = (h * rs) * (w + offset) with rs = fp32(1 / sqrt(mean(h^2)
 // + eps)).  The squares are exact in fp64 and summed there, so rs does not
-// depend on the order of the sum (but within 2e-16 of a rounding border: 5 of
-// 10^10 random rows of fp32 values differ from torch in the last bit of rs), and
-// every later step is one rounded fp32 operation: codes are the same for every
+// depend on the order of the sum, but where it is within some 2e-16 of a border
+// between two fp32 values, which lie 6e-8 to 1.2e-7 apart: a few rows in 10^9.
+// Every later step is one rounded fp32 operation: codes are the same for every
 // launch shape, and equal a plain evaluation's bit for bit.
 //
 // One pass: a row's values stay in registers between the sum, the maximum and
@@ -146,7 +146,8 @@ __device__ __forceinline__ T fold(T v, Op op) {
 // waves' results through LDS (`slot`: a value per wave, used once between
 // barriers; 0 is the operations' identity here).  With lane exchanges through
 // LDS, the waves' results read one by one, and fp64 divisions, the norm of 3
-// rows of 2560 took 4.2 us and that of 4096 24.6; now 3.35 and 22.
+// rows of 2560 took 4.2 us and that of 4096 24.6, and without them 3.35 and 22,
+// both at one chunk per lane (two bring the latter to 18).
 template <class T, class Op>
 __device__ __forceinline__ T row_reduce(T v, int L, T* slot, Op op) {
   v = fold<2>(fold<1>(v, op), op);
@@ -353,9 +354,12 @@ constexpr int kRowMaxH = 32768;                    // 1024 lanes of 4 chunks
 // chunk per lane, the shortest chain: 3 rows of 2560, normed, 3.35 us (2
 // chunks: 3.7).  More rows are bound by the bytes that a CU can have on their
 // way, and take 2 chunks, or 3 where that leaves no more lanes idle and 2 would
-// take more than 4 waves: 16384 rows of 2560, quantized, 25 us (1 chunk: 51, 3:
-// 27); 4096 of 6144, gated, 25.8 (1: 35, 2: 29.5); 3333 of 12000, normed, 57
-// (2: 64).  Rows loaded ahead of the one that is reduced gained nothing.
+// take more than 4 waves: 16384 rows of 2560, quantized, 26 us (1 chunk: 45, 3:
+// 27); 4096 of 6144, gated, 26 (1: 31, 2: 30); 3333 of 12000, normed, 35 (2: 57;
+// 1 does not fit a workgroup).  The rule is coarse for short rows: 8192 of 512,
+// quantized, take 5.6 with a second chunk that only repeats the first one's last
+// (1: 4.9), and 8192 of 1536, normed with a residual, 21.3 (3: 20.1).  Rows loaded
+// ahead of the one that is reduced gained nothing.
 template <int KIND, int TX, int TR, int TW>
 static int launch_row_q8(RowArgs a, hipStream_t st) {
   const int chunks = (a.H + 7) / 8;

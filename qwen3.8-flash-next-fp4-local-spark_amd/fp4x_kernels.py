@@ -199,7 +199,8 @@ def nv4_linear(x2, wp, s, gs, cfg=(32, 256, 4), out_dtype=torch.bfloat16):
 
 
 # ----------------------------------------------------------------- 8-bit activations
-# These functions' checks, outputs and calls are compiled (csrc/fp4x_host.cpp).
+# These functions' checks, outputs and calls are compiled (csrc/fp4x_host.cpp).  Like the linears above they are
+# for inference: their outputs have no gradient, whatever their inputs need.
 def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=False, residual_out=None):
     """Root-mean-square norm of the rows of x [M, H], after the residual's
     addition where one is given, into 8 bits, in one launch.
@@ -238,7 +239,8 @@ def w8a8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
     per output channel (both as quantize_q8 makes them), the sum exact in int32.
     Any M, N and K up to 131071; out_dtype bf16, fp16 or fp32.  Rows that do
     not start on 16 bytes are copied first, which for a weight is worth doing
-    once (quantize_q8 lays its codes out so)."""
+    once (quantize_q8 lays its codes out so).  A bias that is not fp32 is
+    converted in every call, by a launch of its own."""
     return _L.host().w8a8_linear(xq, xs, wq, ws, bias, out_dtype)
 
 
