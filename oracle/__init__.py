@@ -14,6 +14,7 @@ Modules
   hc       hyper-connection mixer rounding points
   head     fast LM head and draft head flows (INT2 coarse -> top-C ->
            exact rescore); coarse sums are exact sums rounded to fp32
+  f8       e4m3 with a scale per block of 128, its product, tokens sorted by expert
   ordered  C replica of the rescore kernels' fma order (bit-exact refined
            logits), float64 exact sums and the MFMA error bound
 

@@ -51,6 +51,17 @@ _SIGS = {
     "fp4x_quantize_q8": ([_P, _I64, _I, _I, _I, _I, _P, _I64, _P, _P], _I),
     "fp4x_w8a8_linear": ([_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _P], _I),
     "fp4x_w8a8_form": ([_I, _I, _I], _I),
+    "fp4x_quantize_f8": ([_P, _I64, _I64, _I, _I, _I, _I, _P, _I64, _I64, _P, _P], _I),
+    "fp4x_f8_linear": ([_P, _I64, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _P], _I),
+    "fp4x_f8_linear_experts": ([_P, _I64, _P, _I64, _I64, _I, _P, _P, _I, _P, _I64, _I64, _P, _P, _I64, _I, _I, _I, _I,
+                                _P], _I),
+    "fp4x_f8_form": ([_I, _I, _I, _I], _I),
+    "fp4x_f8_experts_form": ([_I, _I, _I, _I, _I], _I),
+    "fp4x_expert_sort_workspace": ([_I64, _I, _I], _I64),
+    "fp4x_expert_sort": ([_P, _I, _I64, _I64, _I, _I, _P, _P, _P, _P, _I64, _P], _I),
+    "fp4x_expert_rows": ([_P, _I64, _I, _I, _P, _I, _I, _P, _I64, _P], _I),
+    "fp4x_expert_combine": ([_P, _I64, _I, _I, _P, _P, _I, _P, _I64, _I, _I, _I, _P], _I),
+    "fp4x_expert_combine_grad": ([_P, _I64, _P, _I64, _I, _I, _P, _P, _P, _I, _P, _I64, _P, _I, _I, _I, _P], _I),
     "fp4x_hc_down": ([_P, _I64, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P], _I),
     "fp4x_hc_up": ([_P, _I64, _P, _P, _I, _P, _I64, _P, _I, _I, _I, _I, _I, _P], _I),
     "fp4x_hc_mix": ([_P, _I64, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _P, _I64, _P, _I, _I,
@@ -63,7 +74,7 @@ _SIGS = {
     "fp4x_read_ceiling": ([_P, _I64, _I, _I, _P, _P], _I),
     "fp4x_hold_cus": ([_I, _I64, _I, _P, _P], _I),
 }
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 _LIB = None
 _HOST = None

@@ -1,0 +1,496 @@
+// Tokens sorted by expert and back: expert_sort, expert_rows, expert_combine and
+// its gradient.
+//
+// A router gives each of T tokens k experts' ids.  The T k pairs, sorted by
+// expert and within one by their place (token by token), are the rows of the
+// experts' products: offsets[e] is where expert e's rows begin, tokens[s] the
+// token of row s, slots[t, j] the row of pair (t, j).  Pairs whose id is no
+// expert (negative, or another rank's) have slot -1 and no row; the rows behind
+// the last expert's have token -1.
+//
+// Rows:     r[s] = x[tokens[s]]
+// Combine:  out[t] = sum_j w[t, j] y[slots[t, j]]  (fp32, j in order)
+// Gradient: dy[slots[t, j]] = w[t, j] dout[t],  dw[t, j] = dout[t] . y[slots[t, j]]
+// and the gradient of the rows is the combine without weights.  No atomic decides
+// an order: every result is the same in every run.
+#include <algorithm>
+#include <string>
+
+#include "fp4x_f8.h"
+#include "../../include/fp4x.h"
+
+namespace fp4x {
+
+static int ex_fail(const char* what, const char* why) {
+  set_error(std::string(what) + ": " + why);
+  return FP4X_ERR_ARG;
+}
+
+// ------------------------------------------------------------------ sort
+// A counting sort.  A workgroup takes a chunk of consecutive pairs, each of its
+// waves a part of that: counts per wave and expert in LDS, their sums over the
+// waves before, and then every wave walks its pairs again, 64 at a time, and
+// gives each the next place of its expert; within the 64 a pair's place is the
+// number of lanes before it with the same id.
+//
+// Up to kSortOne pairs one workgroup does all.  Above, a first launch counts
+// per chunk, and in the second each workgroup adds up the chunks before its own
+// and the totals (at most 256 chunks of E counts, from L2).
+constexpr int kSortOne = 4096, kSortChunks = 256, kSortLds = 128 * 1024;
+
+struct SortArgs {
+  const void* ids;  int wide;  int64_t row;        // int64 or int32, elements between tokens
+  int P, k, E, W, chunk, chunks;                   // W: waves per workgroup
+  int* hist;                                       // [chunks][E]
+  int *offsets, *tokens, *slots;
+};
+
+__device__ __forceinline__ int sort_id(const SortArgs& a, int p) {   // E: none
+  const int t = (int)((unsigned)p / (unsigned)a.k);
+  const int64_t at = t * a.row + (p - t * a.k);
+  const int64_t id = a.wide ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
+  return id >= 0 && id < a.E ? (int)id : a.E;
+}
+// Counts of this chunk's pairs per wave and expert.
+__device__ __forceinline__ void sort_count(const SortArgs& a, int p0, int p1, int* cnt) {
+  for (int i = threadIdx.x; i < a.W * a.E; i += 64 * a.W) cnt[i] = 0;
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int p = p0 + lane; p < p1; p += 64) {
+    const int id = sort_id(a, p);
+    if (id < a.E) atomicAdd(&cnt[wave * a.E + id], 1);
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void sort_part(const SortArgs& a, int chunk, int& p0, int& p1) {
+  const int per = ((a.chunk + a.W - 1) / a.W + 63) & -64, wave = threadIdx.x >> 6;
+  const int64_t c0 = (int64_t)chunk * a.chunk, end = min(c0 + a.chunk, (int64_t)a.P), lo = c0 + (int64_t)wave * per;
+  p0 = (int)min(lo, end);
+  p1 = (int)min(lo + per, end);
+}
+
+__global__ __launch_bounds__(1024) void sort_count_kernel(const SortArgs a) {
+  extern __shared__ int cnt[];
+  int p0, p1;
+  sort_part(a, blockIdx.x, p0, p1);
+  sort_count(a, p0, p1, cnt);
+  for (int e = threadIdx.x; e < a.E; e += 64 * a.W) {
+    int n = 0;
+    for (int w = 0; w < a.W; ++w) n += cnt[w * a.E + e];
+    a.hist[(int64_t)blockIdx.x * a.E + e] = n;
+  }
+}
+
+__global__ __launch_bounds__(1024) void sort_place_kernel(const SortArgs a) {
+  extern __shared__ int cnt[];
+  __shared__ int wave_total[16];
+  int p0, p1;
+  sort_part(a, blockIdx.x, p0, p1);
+  sort_count(a, p0, p1, cnt);
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, threads = 64 * a.W;
+  int carry = 0;
+  for (int e0 = 0; e0 < a.E; e0 += threads) {      // a thread per expert
+    const int e = e0 + t;
+    int before = 0, total = 0, own = 0;
+    if (e < a.E) {
+      for (int w = 0; w < a.W; ++w) {
+        const int n = cnt[w * a.E + e];
+        cnt[w * a.E + e] = own;
+        own += n;
+      }
+      if (a.chunks == 1) {
+        total = own;
+      } else {
+#pragma unroll 8
+        for (int c = 0; c < a.chunks; ++c) {
+          const int n = a.hist[(int64_t)c * a.E + e];
+          total += n;
+          if (c < (int)blockIdx.x) before += n;
+        }
+      }
+    }
+    const int upto = wave_sum_to(total);
+    if (lane == 63) wave_total[wave] = upto;
+    __syncthreads();
+    int base = carry;
+    for (int w = 0; w < a.W; ++w) {
+      const int n = wave_total[w];
+      if (w < wave) base += n;
+      carry += n;
+    }
+    base += upto - total;                          // where expert e begins
+    if (e < a.E) {
+      if (blockIdx.x == 0) a.offsets[e] = base;
+      for (int w = 0; w < a.W; ++w) cnt[w * a.E + e] += base + before;
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && t == 0) a.offsets[a.E] = carry;
+  volatile int* next = cnt + wave * a.E;           // (a wave's LDS operations are done in order)
+  for (int p = p0 + lane; p - lane < p1; p += 64) {
+    const int id = p < p1 ? sort_id(a, p) : a.E;
+    const bool has = id < a.E;
+    uint64_t same = __ballot(has);
+    for (int b = 0; b < 32 - __builtin_clz(a.E); ++b) {
+      const uint64_t m = __ballot(has && (id >> b & 1));
+      same &= id >> b & 1 ? m : ~m;
+    }
+    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+    if (has) {
+      const int at = next[id];
+      if (rank == 0) next[id] = at + __popcll(same);
+      a.tokens[at + rank] = (int)((unsigned)p / (unsigned)a.k);
+      a.slots[p] = at + rank;
+    } else if (p < p1) {
+      a.slots[p] = -1;
+    }
+  }
+  for (int64_t s = carry + (int64_t)blockIdx.x * threads + t; s < a.P; s += (int64_t)gridDim.x * threads) a.tokens[s] = -1;
+}
+
+// ------------------------------------------------------------------ rows
+// Bytes are copied as they are, 16 at a time, the last 16 of a row again where
+// its length is no multiple.  A wave takes up to kRowPart bytes of a row.
+constexpr int kRowPart = 8192;
+typedef uint32_t u32x4_b __attribute__((ext_vector_type(4), aligned(1)));
+
+struct RowsArgs {
+  const uint8_t* x;  int64_t x_stride;             // bytes
+  const int* tokens;
+  uint8_t* out;  int64_t out_stride;
+  int T, P, parts;
+  int64_t bytes;
+};
+__global__ __launch_bounds__(256) void expert_rows_kernel(const RowsArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t waves = (int64_t)gridDim.x * 4, items = (int64_t)a.P * a.parts;
+  for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += waves) {
+    const int64_t s = it / a.parts, b0 = (it - s * a.parts) * kRowPart, n = min(a.bytes - b0, (int64_t)kRowPart);
+    const int tok = a.tokens[s];
+    const bool has = tok >= 0 && tok < a.T;
+    const uint8_t* from = a.x + (int64_t)(has ? tok : 0) * a.x_stride + b0;
+    uint8_t* to = a.out + s * a.out_stride + b0;
+    if (n < 16) {
+      if (lane < n) to[lane] = has ? from[lane] : 0;
+      continue;
+    }
+    u32x4_b v[kRowPart / 1024];
+#pragma unroll
+    for (int i = 0; i < kRowPart / 1024; ++i) {
+      const int64_t at = (i * 64 + lane) * 16;
+      v[i] = u32x4_b{0, 0, 0, 0};
+      if (has && i * 1024 < n) v[i] = *reinterpret_cast<const u32x4_b*>(from + min(at, n - 16));
+    }
+#pragma unroll
+    for (int i = 0; i < kRowPart / 1024; ++i) {
+      const int64_t at = (i * 64 + lane) * 16;
+      if (at < n) *reinterpret_cast<u32x4_b*>(to + min(at, n - 16)) = v[i];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ combine
+typedef uint32_t u32x4_e __attribute__((ext_vector_type(4), aligned(2)));
+
+template <int DT> struct Vec8;                     // eight values of a type, as loaded
+template <> struct Vec8<DT_F32> {
+  u32x4_e a, b;
+  __device__ void load(const void* p, int64_t i) {
+    const u32x4_e* g = reinterpret_cast<const u32x4_e*>(static_cast<const float*>(p) + i);
+    a = g[0];
+    b = g[1];
+  }
+  __device__ float get(int j) const { return __uint_as_float(j < 4 ? a[j] : b[j - 4]); }
+};
+template <int DT> struct Vec8 {
+  u32x4_e v;
+  __device__ void load(const void* p, int64_t i) { v = *reinterpret_cast<const u32x4_e*>(static_cast<const uint16_t*>(p) + i); }
+  __device__ float get(int j) const {
+    const uint32_t d = v[j >> 1];
+    if constexpr (DT == DT_BF16) return j & 1 ? bf16_hi(d) : bf16_lo(d);
+    else return f16_to_f32((uint16_t)(j & 1 ? d >> 16 : d));
+  }
+};
+template <int DT>
+__device__ __forceinline__ void put8(void* p, int64_t i, const float (&f)[8]) {
+  if constexpr (DT == DT_F32) {
+    u32x4_e* g = reinterpret_cast<u32x4_e*>(static_cast<float*>(p) + i);
+    g[0] = u32x4_e{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    g[1] = u32x4_e{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
+  } else {
+    uint32_t d[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      d[j] = DT == DT_BF16 ? pack_bf16x2(f[2 * j], f[2 * j + 1]) : pack_f16x2(f[2 * j], f[2 * j + 1]);
+    *reinterpret_cast<u32x4_e*>(static_cast<uint16_t*>(p) + i) = u32x4_e{d[0], d[1], d[2], d[3]};
+  }
+}
+template <int DT>
+__device__ __forceinline__ float get1(const void* p, int64_t i) {
+  if constexpr (DT == DT_F32) return static_cast<const float*>(p)[i];
+  else if constexpr (DT == DT_BF16) return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
+  else return f16_to_f32(static_cast<const uint16_t*>(p)[i]);
+}
+__device__ __forceinline__ float weight_at(const void* w, int dt, int64_t i) {
+  return dt == DT_F32 ? get1<DT_F32>(w, i) : dt == DT_BF16 ? get1<DT_BF16>(w, i) : get1<DT_F16>(w, i);
+}
+
+struct CombineArgs {
+  const void* y;  int64_t y_stride;
+  const int* slots;
+  const void* w;  int w_dtype;                     // [T, k] or null
+  void* out;  int64_t out_stride;
+  int T, k, P, H, parts;                           // parts: waves per token
+};
+
+// A wave takes 512 values of a token, eight per lane, and its k rows eight at a time, whose loads are on their way
+// together.  The last lanes of a row are moved back to end at H.
+template <int DT>
+__global__ __launch_bounds__(256) void expert_combine_kernel(const CombineArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t waves = (int64_t)gridDim.x * 4, items = (int64_t)a.T * a.parts;
+  for (int64_t it = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); it < items; it += waves) {
+    const int64_t t = it / a.parts;
+    const int h0 = ((int)(it - t * a.parts) * 64 + lane) * 8;
+    const int* slots = a.slots + t * a.k;
+    if (a.H < 8) {
+      if (lane < a.H) {
+        float acc = 0.0f;
+        for (int j = 0; j < a.k; ++j) {
+          const int s = slots[j];
+          if (s >= 0 && s < a.P)
+            acc = __builtin_fmaf(a.w ? weight_at(a.w, a.w_dtype, t * a.k + j) : 1.0f, get1<DT>(a.y, s * a.y_stride + lane), acc);
+        }
+        store_out(a.out, t * a.out_stride + lane, DT, acc);
+      }
+      continue;
+    }
+    const int h = min(h0, a.H - 8);
+    float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j0 = 0; j0 < a.k; j0 += 8) {
+      Vec8<DT> v[8];
+      float w[8];
+      bool has[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = min(j0 + j, a.k - 1), s = slots[at];
+        has[j] = j0 + j < a.k && s >= 0 && s < a.P;
+        if (has[j]) v[j].load(a.y, s * a.y_stride + h);
+        w[j] = a.w ? weight_at(a.w, a.w_dtype, t * a.k + at) : 1.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (has[j])
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w[j], v[j].get(i), acc[i]);
+    }
+    if (h0 < a.H) put8<DT>(a.out, t * a.out_stride + h, acc);
+  }
+}
+
+// ------------------------------------------------------------------ its gradient
+constexpr int kGradTop = 128, kGradTail = 64;      // pairs per token; rows that a workgroup of the second role looks at
+
+struct GradArgs {
+  const void* d;  int64_t d_stride;                // dout
+  const void* y;  int64_t y_stride;
+  const int *slots, *tokens;
+  const void* w;  int w_dtype;
+  void* dy;  int64_t dy_stride;
+  void* dw;
+  int T, k, P, H;
+};
+
+// A workgroup takes a token: its row of dout stays in registers, C chunks of
+// eight values per lane, while its k rows of y go by.  A wave's sum of the
+// products is a butterfly, the waves' are added in their order.  Workgroups past
+// the tokens clear the rows that no pair has.
+template <int DT, int C>
+__global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
+  __shared__ float sum[16][kGradTop];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), W = blockDim.x >> 6;
+  if ((int)blockIdx.x >= a.T) {
+    const int64_t s0 = (int64_t)(blockIdx.x - a.T) * kGradTail, s1 = min(s0 + kGradTail, (int64_t)a.P);
+    for (int64_t s = s0; s < s1; ++s) {
+      const int tok = a.tokens[s];
+      if (tok >= 0 && tok < a.T) continue;
+      for (int h = t; h < a.H; h += blockDim.x) store_out(a.dy, s * a.dy_stride + h, DT, 0.0f);
+    }
+    return;
+  }
+  const int64_t tok = blockIdx.x;
+  const int* slots = a.slots + tok * a.k;
+  if (a.H < 8) {                                   // (one wave)
+    const float d = lane < a.H ? get1<DT>(a.d, tok * a.d_stride + lane) : 0.0f;
+    for (int j = 0; j < a.k; ++j) {
+      const int s = slots[j];
+      const bool has = s >= 0 && s < a.P;
+      float v = 0.0f;
+      if (has && lane < a.H) {
+        v = d * get1<DT>(a.y, s * a.y_stride + lane);
+        store_out(a.dy, s * a.dy_stride + lane, DT, weight_at(a.w, a.w_dtype, tok * a.k + j) * d);
+      }
+      v = group_allreduce(v, 64);
+      if (lane == 0) store_out(a.dw, tok * a.k + j, a.w_dtype, v);
+    }
+    return;
+  }
+  int h[C];
+  bool in[C];
+  Vec8<DT> d[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int h0 = (c * (int)blockDim.x + t) * 8;
+    in[c] = h0 < a.H;
+    h[c] = min(h0, a.H - 8);
+    d[c].load(a.d, tok * a.d_stride + h[c]);
+  }
+  for (int j = 0; j < a.k; ++j) {
+    const int s = slots[j];
+    float dot = 0.0f;
+    if (s >= 0 && s < a.P) {
+      const float w = weight_at(a.w, a.w_dtype, tok * a.k + j);
+      Vec8<DT> v[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[c].load(a.y, s * a.y_stride + h[c]);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int dup = (c * (int)blockDim.x + t) * 8 - h[c];   // values that the chunk before has, of one moved back
+        float g[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          g[i] = w * d[c].get(i);
+          if (in[c] && i >= dup) dot = __builtin_fmaf(d[c].get(i), v[c].get(i), dot);
+        }
+        if (in[c]) put8<DT>(a.dy, s * a.dy_stride + h[c], g);
+      }
+    }
+    dot = group_allreduce(dot, 64);
+    if (lane == 0) sum[wave][j] = dot;
+  }
+  __syncthreads();
+  for (int j = t; j < a.k; j += blockDim.x) {
+    float v = sum[0][j];
+    for (int q = 1; q < W; ++q) v += sum[q][j];
+    store_out(a.dw, tok * a.k + j, a.w_dtype, v);
+  }
+}
+
+template <int DT>
+static void launch_grad(const GradArgs& a, hipStream_t st) {
+  const int chunks = (a.H + 7) / 8, C = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 4;
+  const int threads = std::min(1024, ((chunks + C - 1) / C + 63) / 64 * 64);
+  const dim3 grid((unsigned)(a.T + (a.P + (int64_t)kGradTail - 1) / kGradTail));
+  if (C == 1) hipLaunchKernelGGL((expert_grad_kernel<DT, 1>), grid, dim3(threads), 0, st, a);
+  else if (C == 2) hipLaunchKernelGGL((expert_grad_kernel<DT, 2>), grid, dim3(threads), 0, st, a);
+  else hipLaunchKernelGGL((expert_grad_kernel<DT, 4>), grid, dim3(threads), 0, st, a);
+}
+
+static bool ex_dt(int dt) { return dt == DT_BF16 || dt == DT_F32 || dt == DT_F16; }
+static bool ex_al(const void* p, int dt) { return (reinterpret_cast<uintptr_t>(p) & (dt == DT_F32 ? 3 : 1)) == 0; }
+static bool al4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+}  // namespace fp4x
+
+using namespace fp4x;
+
+extern "C" {
+
+int64_t fp4x_expert_sort_workspace(int64_t T, int k, int E) {
+  const int64_t P = T * k;
+  if (P <= kSortOne) return 0;
+  const int64_t chunk = std::max<int64_t>(kSortOne, ((P + kSortChunks - 1) / kSortChunks + 1023) / 1024 * 1024);
+  return (P + chunk - 1) / chunk * E * (int64_t)sizeof(int);
+}
+
+int fp4x_expert_sort(const void* ids, int wide, int64_t row, int64_t T, int k, int E, int* offsets, int* tokens,
+                     int* slots, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "expert_sort";
+  if (T < 0 || k < 1 || k > 1 << 20 || E < 1 || E > kF8MaxExperts) return ex_fail(what, "need T >= 0, 1 <= k <= 2^20 and 1 to 4096 experts");
+  if (T > (1 << 30) / k) return ex_fail(what, "more than 2^30 pairs");
+  if (!offsets || !al4(offsets)) return ex_fail(what, "null or misaligned offsets");
+  if (T && (!ids || !tokens || !slots)) return ex_fail(what, "null ids, tokens or slots");
+  if ((reinterpret_cast<uintptr_t>(ids) & (wide ? 7 : 3)) || !al4(tokens) || !al4(slots))
+    return ex_fail(what, "tensors must be aligned to their element");
+  if (row < 0) return ex_fail(what, "a stride is negative");
+  const int64_t need = fp4x_expert_sort_workspace(T, k, E);
+  if (need && (!workspace || workspace_bytes < need || !al4(workspace))) return ex_fail(what, "the workspace is too small, null or misaligned");
+  const int P = (int)(T * k);
+  int W = std::min(16, std::max(1, kSortLds / 4 / E));
+  if (P <= 2048) W = std::min(W, std::max(1, (P + 255) / 256 * 2));       // few pairs: few counts to clear and to add
+  SortArgs a{ids, wide ? 1 : 0, row, P, k, E, W, 0, 1, static_cast<int*>(workspace), offsets, tokens, slots};
+  hipStream_t st = (hipStream_t)stream;
+  if (need) {
+    a.chunk = std::max(kSortOne, ((P + kSortChunks - 1) / kSortChunks + 1023) / 1024 * 1024);
+    a.chunks = (P + a.chunk - 1) / a.chunk;
+  } else {
+    a.chunk = (std::max(P, 1) + 64 * W - 1) / (64 * W) * (64 * W);
+  }
+  const int lds = W * E * (int)sizeof(int);
+  if (lds > 48 * 1024) {
+    for (const void* f : {reinterpret_cast<const void*>(sort_count_kernel), reinterpret_cast<const void*>(sort_place_kernel)})
+      if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return check_launch(what);
+  }
+  if (need) hipLaunchKernelGGL(sort_count_kernel, dim3(a.chunks), dim3(64 * W), lds, st, a);
+  hipLaunchKernelGGL(sort_place_kernel, dim3(a.chunks), dim3(64 * W), lds, st, a);
+  return check_launch(what);
+}
+
+int fp4x_expert_rows(const void* x, int64_t x_stride, int elem, int T, const int* tokens, int P, int H, void* out,
+                     int64_t out_stride, void* stream) {
+  const char* what = "expert_rows";
+  if (T < 0 || P < 0 || H < 1 || (elem != 1 && elem != 2 && elem != 4)) return ex_fail(what, "need T and P >= 0, H >= 1 and elements of 1, 2 or 4 bytes");
+  if (P == 0) return FP4X_OK;
+  if ((!x && T) || !tokens || !out || !al4(tokens)) return ex_fail(what, "null tensor, or misaligned tokens");
+  if (x_stride < 0 || (P > 1 && out_stride < H)) return ex_fail(what, "output rows overlap, or a stride is negative");
+  const int64_t bytes = (int64_t)H * elem;
+  const int64_t parts = (bytes + kRowPart - 1) / kRowPart;
+  const RowsArgs a{static_cast<const uint8_t*>(x), x_stride * elem, tokens, static_cast<uint8_t*>(out), out_stride * elem,
+                   T, P, (int)parts, bytes};
+  const dim3 grid((unsigned)std::min<int64_t>((P * parts + 3) / 4, 1 << 20));
+  hipLaunchKernelGGL(expert_rows_kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
+  return check_launch(what);
+}
+
+int fp4x_expert_combine(const void* y, int64_t y_stride, int dtype, int P, const int* slots, const void* w, int w_dtype,
+                        void* out, int64_t out_stride, int T, int k, int H, void* stream) {
+  const char* what = "expert_combine";
+  if (!ex_dt(dtype) || (w && !ex_dt(w_dtype))) return ex_fail(what, "rows and weights are bf16, fp16 or fp32");
+  if (T < 0 || k < 1 || P < 0 || H < 1) return ex_fail(what, "need T and P >= 0, k and H >= 1");
+  if (T == 0) return FP4X_OK;
+  if ((!y && P) || !slots || !out || !al4(slots) || !ex_al(y, dtype) || !ex_al(out, dtype) || (w && !ex_al(w, w_dtype)))
+    return ex_fail(what, "null tensor, or one that is not aligned to its element");
+  if (y_stride < 0 || (T > 1 && out_stride < H)) return ex_fail(what, "output rows overlap, or a stride is negative");
+  const int parts = (H + 511) / 512;
+  const CombineArgs a{y, y_stride, slots, w, w_dtype, out, out_stride, T, k, P, H, parts};
+  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)T * parts + 3) / 4, 1 << 20));
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_BF16) hipLaunchKernelGGL((expert_combine_kernel<DT_BF16>), grid, dim3(256), 0, st, a);
+  else if (dtype == DT_F16) hipLaunchKernelGGL((expert_combine_kernel<DT_F16>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((expert_combine_kernel<DT_F32>), grid, dim3(256), 0, st, a);
+  return check_launch(what);
+}
+
+int fp4x_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int dtype, int P,
+                             const int* slots, const int* tokens, const void* w, int w_dtype, void* dy,
+                             int64_t dy_stride, void* dw, int T, int k, int H, void* stream) {
+  const char* what = "expert_combine_grad";
+  if (!ex_dt(dtype) || !ex_dt(w_dtype)) return ex_fail(what, "rows and weights are bf16, fp16 or fp32");
+  if (T < 0 || k < 1 || k > kGradTop || P < 0 || H < 1 || H > 32768)
+    return ex_fail(what, "need T and P >= 0, 1 <= k <= 128 and 1 <= H <= 32768");
+  if (T == 0 && P == 0) return FP4X_OK;
+  if ((T && (!dout || !slots || !w || !dw)) || (P && (!y || !tokens || !dy))) return ex_fail(what, "null tensor");
+  if (!al4(slots) || !al4(tokens) || !ex_al(dout, dtype) || !ex_al(y, dtype) || !ex_al(dy, dtype) || !ex_al(w, w_dtype) ||
+      !ex_al(dw, w_dtype))
+    return ex_fail(what, "tensors must be aligned to their element");
+  if (dout_stride < 0 || y_stride < 0 || (P > 1 && dy_stride < H)) return ex_fail(what, "output rows overlap, or a stride is negative");
+  if (T + ((int64_t)P + kGradTail - 1) / kGradTail > INT32_MAX) return ex_fail(what, "too many rows");
+  const GradArgs a{dout, dout_stride, y, y_stride, slots, tokens, w, w_dtype, dy, dy_stride, dw, T, k, P, H};
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_BF16) launch_grad<DT_BF16>(a, st);
+  else if (dtype == DT_F16) launch_grad<DT_F16>(a, st);
+  else launch_grad<DT_F32>(a, st);
+  return check_launch(what);
+}
+
+}  // extern "C"

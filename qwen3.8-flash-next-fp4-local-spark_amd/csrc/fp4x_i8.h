@@ -37,18 +37,21 @@ struct I8Run {
   __device__ I8Run(int tiles, int xcd) : first(xcd * (tiles >> 3) + min(xcd, tiles & 7)),
                                          count((tiles >> 3) + (xcd < (tiles & 7))) {}
 };
-__device__ __forceinline__ void i8_place(const I8Args& a, int id, int bm, int bn, int& m0, int& n0) {
-  int band = 0, r = id, h = a.mt;
-  if (a.mt > a.gm) {
-    const int per = a.gm * a.nt;
+__device__ __forceinline__ void tile_place(int mt, int nt, int gm, int id, int bm, int bn, int& m0, int& n0) {
+  int band = 0, r = id, h = mt;
+  if (mt > gm) {
+    const int per = gm * nt;
     band = id / per;
     r = id - band * per;
-    h = min(a.gm, a.mt - band * a.gm);
+    h = min(gm, mt - band * gm);
   }
   // (no general division for the heights of a band and of few rows)
   const int n = h == 1 ? r : h == 2 ? r >> 1 : h == 3 ? (int)__umulhi(r, 0x55555556u) : h == 4 ? r >> 2 : r / h;
-  m0 = (band * a.gm + r - n * h) * bm;
+  m0 = (band * gm + r - n * h) * bm;
   n0 = n * bn;
+}
+__device__ __forceinline__ void i8_place(const I8Args& a, int id, int bm, int bn, int& m0, int& n0) {
+  tile_place(a.mt, a.nt, a.gm, id, bm, bn, m0, n0);
 }
 
 // Direct loads to LDS: lane l's 16 (4) bytes at base + off land at lds + 16 l

@@ -5,7 +5,10 @@
 //   e4m3  s = max(amax, 1e-12) / 448, q = e4m3fn(v / s), one fp32 s per row
 //   mx8   per 32 values the exponent X = clamp(floor(log2 amax) - 8, -127,
 //         127) as the byte X + 127, q = e4m3fn(v * 2^-X) saturating at 448
-// with IEEE fp32 division and round half to even.  A row (mx8: a block of 32)
+//   e4m3_g128  as e4m3 for each 128 values (the row's last block may be
+//         shorter): fp32 scales [M, ceil(H / 128)], those of a block side by side
+//         in memory, as f8_linear's tiles read them
+// with IEEE fp32 division and round half to even.  A row (mx8: a block of 32, e4m3_g128: of 128)
 // that holds an infinity or a NaN gets the scale NaN (byte 255) and the codes
 // 0 (mx8: NaN codes), so that one bad token stays one bad row.
 //
@@ -34,7 +37,7 @@ namespace fp4x {
 int device_cus();
 
 enum RowKind : int { ROW_NORM, ROW_SILU, ROW_QUANT };
-enum RowFmt : int { ROW_INT8, ROW_E4M3, ROW_MX8 };
+enum RowFmt : int { ROW_INT8 = FP4X_Q8_INT8, ROW_E4M3 = FP4X_Q8_E4M3, ROW_MX8 = FP4X_Q8_MX8, ROW_G128 = FP4X_Q8_E4M3_G128 };
 
 struct RowArgs {
   const void* x;  int64_t x_stride;                // rows (the gate)
@@ -181,6 +184,22 @@ __device__ __forceinline__ uint32_t e4m3x4(const float* f) {
   int d = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], d, true);
 }
+// e4m3(f / s) of eight values with one scale; `quick` where every lane's s allows the quotient from the reciprocal.
+__device__ __forceinline__ void e4m3_codes(const float (&f)[8], float s, bool quick, uint32_t& lo, uint32_t& hi) {
+  float g[8];
+  if (quick) {
+    const float rc = 1.0f / s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = exact_quot(f[j], s, rc);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = f[j] / s;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) g[j] = copysignf(fminf(fabsf(g[j]), 448.0f), f[j]);   // -0 too
+  lo = e4m3x4(g);
+  hi = e4m3x4(g + 4);
+}
 __device__ __forceinline__ void store_codes(uint8_t* q, uint32_t lo, uint32_t hi, int n) {
   if (n >= 8) {
     *reinterpret_cast<u32x2_any*>(q) = u32x2_any{lo, hi};
@@ -304,6 +323,34 @@ __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
           if ((l & 3) == 0) static_cast<uint8_t*>(a.s)[row * (a.H / 32) + k[c] / 32] = fin ? (uint8_t)(X + 127) : 255;
         }
       }
+    } else if (a.fmt == ROW_G128) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int d = (c * L + l) * 8 - k[c];      // duplicates at the front of a chunk moved back: of the block before
+        float b = m[c];
+        if (d > 0) {
+          b = 0.0f;
+#pragma unroll
+          for (int j = 1; j < 8; ++j) b = j >= d ? __builtin_elementwise_maximum(b, fabsf(f[c][j])) : b;
+        }
+        b = fold<2>(fold<1>(b, MaxF32()), MaxF32());   // 16 lanes hold a block (all of a row of fewer)
+        if (L > 4) b = fold<4>(b, MaxF32());
+        if (L > 8) b = fold<8>(b, MaxF32());
+        const bool fin = b < __builtin_inff();
+        const float s = fmaxf(b, 1e-12f) / 448.0f;
+        uint32_t lo, hi;
+        e4m3_codes(f[c], s, __all(fin && mid_range(s)), lo, hi);
+        if (!fin) lo = hi = 0;
+        const int at = c * L + l;
+        if (live && at * 8 < a.H) {
+          uint8_t* q = a.q + row * a.q_stride + k[c];
+          if (d == 0) store_codes(q, lo, hi, n);
+          else
+            for (int j = d; j < 8; ++j) q[j] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+          if ((l & 15) == 0)
+            static_cast<float*>(a.s)[(int64_t)(at >> 4) * a.M + row] = fin ? s : __uint_as_float(0x7fc00000u);
+        }
+      }
     } else {
       float amax = m[0];
 #pragma unroll
@@ -344,6 +391,59 @@ __global__ __launch_bounds__(1024) void row_q8_kernel(const RowArgs a) {
       if (live && l == 0) static_cast<float*>(a.s)[row] = fin ? s : __uint_as_float(0x7fc00000u);
     }
     if (L > 64) __syncthreads();                   // the slots are used again
+  }
+}
+
+// A weight in e4m3 with a scale per 128 x 128 block (blocks at its ends may be
+// smaller), [E, N, K]: the values of a block stay in the registers of one
+// workgroup, 8 rows x 8 values per lane, between the maximum and the codes.
+struct BlockArgs {
+  const void* w;  int64_t w_row, w_expert;         // strides in elements
+  uint8_t* q;  int64_t q_row, q_expert;            // strides in bytes
+  float* s;
+  int N, K, nb, kb;
+  int64_t blocks;
+};
+template <int T>
+__global__ __launch_bounds__(256) void block_q8_kernel(const BlockArgs a) {
+  __shared__ float slot[4];
+  const int t = threadIdx.x, r0 = t >> 4;
+  for (int64_t b = blockIdx.x; b < a.blocks; b += gridDim.x) {
+    const int64_t bn = b / a.kb;
+    const int e = (int)(bn / a.nb), n0 = (int)(bn % a.nb) * 128, k0 = (int)(b % a.kb) * 128 + (t & 15) * 8;
+    const int nk = min(max(a.K - k0, 0), 8);
+    float f[8][8], m = 0.0f;
+    Raw8<T> raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t at = e * a.w_expert + min(n0 + r0 + 16 * i, a.N - 1) * a.w_row + k0;
+      if (nk == 8) raw[i].load(a.w, at);
+      else raw[i].load_n(a.w, at, nk);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {                  // (rows past the end hold the last one's values)
+      raw[i].get(f[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = __builtin_elementwise_maximum(m, fabsf(f[i][j]));
+    }
+    m = fold<8>(fold<4>(fold<2>(fold<1>(m, MaxF32()), MaxF32()), MaxF32()), MaxF32());
+    m = fold<32>(fold<16>(m, MaxF32()), MaxF32());
+    if ((t & 63) == 0) slot[t >> 6] = m;
+    __syncthreads();
+    m = slot[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_maximum(m, slot[i]);
+    const bool fin = m < __builtin_inff();
+    const float s = fmaxf(m, 1e-12f) / 448.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t lo, hi;
+      e4m3_codes(f[i], s, fin && mid_range(s), lo, hi);
+      if (!fin) lo = hi = 0;
+      if (n0 + r0 + 16 * i < a.N) store_codes(a.q + e * a.q_expert + (n0 + r0 + 16 * i) * a.q_row + k0, lo, hi, nk);
+    }
+    if (t == 0) a.s[b] = fin ? s : __uint_as_float(0x7fc00000u);
+    __syncthreads();                               // the slots are used again
   }
 }
 
@@ -426,7 +526,7 @@ static bool known_dt(int dt) { return dt == DT_BF16 || dt == DT_F32 || dt == DT_
 static int row_check(const char* what, const RowArgs& a, int dtype) {
   if (!known_dt(dtype)) return row_fail(what, "rows are bf16, fp16 or fp32");
   if (a.M < 0 || a.H < 1 || a.H > kRowMaxH) return row_fail(what, "need M >= 0 and 1 <= H <= 32768");
-  if (a.fmt < ROW_INT8 || a.fmt > ROW_MX8) return row_fail(what, "unknown format");
+  if (a.fmt != ROW_INT8 && a.fmt != ROW_E4M3 && a.fmt != ROW_MX8 && a.fmt != ROW_G128) return row_fail(what, "unknown format");
   if (a.fmt == ROW_MX8 && a.H % 32) return row_fail(what, "mx8 needs rows of a multiple of 32 values");
   if (a.M == 0) return FP4X_OK;
   if (!a.x || !a.q || !a.s) return row_fail(what, "null rows, codes or scales");
@@ -505,6 +605,26 @@ int fp4x_quantize_q8(const void* x, int64_t x_stride, int dtype, int M, int H, i
   if (dtype == DT_BF16) return launch_row_q8<ROW_QUANT, DT_BF16, DT_BF16, DT_BF16>(a, st);
   if (dtype == DT_F16) return launch_row_q8<ROW_QUANT, DT_F16, DT_F16, DT_F16>(a, st);
   return launch_row_q8<ROW_QUANT, DT_F32, DT_F32, DT_F32>(a, st);
+}
+
+int fp4x_quantize_f8(const void* w, int64_t w_row, int64_t w_expert, int dtype, int E, int N, int K, void* q, int64_t q_row,
+                     int64_t q_expert, float* s, void* stream) {
+  const char* what = "quantize_f8";
+  if (!known_dt(dtype)) return row_fail(what, "weights are bf16, fp16 or fp32");
+  if (E < 0 || N < 0 || K < 1 || N > 1 << 24 || K > 1 << 24) return row_fail(what, "need E and N >= 0, K >= 1, N and K up to 2^24");
+  if (E == 0 || N == 0) return FP4X_OK;
+  if (!w || !q || !s) return row_fail(what, "null weight, codes or scales");
+  if (!el_aligned(w, dtype) || (reinterpret_cast<uintptr_t>(s) & 3)) return row_fail(what, "weights and scales must be aligned to their element");
+  if (w_row < 0 || w_expert < 0 || q_row < K || (E > 1 && q_expert < (N - 1) * q_row + K))
+    return row_fail(what, "the code rows overlap, or a stride is negative");
+  const int nb = (N + 127) / 128, kb = (K + 127) / 128;
+  const BlockArgs a{w, w_row, w_expert, static_cast<uint8_t*>(q), q_row, q_expert, s, N, K, nb, kb, (int64_t)E * nb * kb};
+  const dim3 grid((unsigned)std::min<int64_t>(a.blocks, 1 << 20));
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_BF16) hipLaunchKernelGGL((block_q8_kernel<DT_BF16>), grid, dim3(256), 0, st, a);
+  else if (dtype == DT_F16) hipLaunchKernelGGL((block_q8_kernel<DT_F16>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((block_q8_kernel<DT_F32>), grid, dim3(256), 0, st, a);
+  return check_launch(what);
 }
 
 }  // extern "C"

@@ -26,6 +26,8 @@ __all__ = [
     "mx8_linear", "bf16_linear", "nv4_linear", "w8_linear", "w6_linear", "int2_logits", "refine_mx8_", "refine_nv4",
     "scatter_draft", "draft_nv4",
     "rms_norm_q8", "silu_mul_q8", "quantize_q8", "w8a8_linear",
+    "quantize_f8", "f8_linear", "f8_linear_experts",
+    "expert_sort", "expert_rows", "expert_combine", "expert_combine_grad",
     "topk_rows", "int2_topk", "w8_linear_layers", "HCFused", "hc_scaled_silu", "hc_gate_mean",
     "quantize_w8", "quantize_w6", "quantize_nv4", "quantize_int2", "quantize_mx8",
     "mx8_dequant", "dequant_int2", "dequant_nv4", "dequant_operand", "requantize_mx8", "requantize_nv4", "ORDER",
@@ -213,8 +215,10 @@ def rms_norm_q8(x, w, eps=1e-6, residual=None, fmt="int8", w_offset=0.0, normed=
 
     fmt "int8": int8 codes and fp32 scales [M] (w8a8_linear takes them);
     "e4m3": the same with float8_e4m3fn codes; "mx8": MXFP8, float8_e4m3fn
-    codes and uint8 e8m0 scales [M, H/32].  A row (mx8: a block) with an
-    infinity or a NaN gets the scale NaN.  x is bf16, fp16 or fp32; residual
+    codes and uint8 e8m0 scales [M, H/32]; "e4m3_g128": float8_e4m3fn codes
+    and fp32 scales [M, ceil(H/128)], one per 128 values, a block's side by
+    side in memory (f8_linear takes them).  A row (mx8 and e4m3_g128: a block)
+    with an infinity or a NaN gets the scale NaN.  x is bf16, fp16 or fp32; residual
     and w have its type or are fp32.  1 <= H <= 32768.  q and s of up to 1 MiB
     together share one storage."""
     return _L.host().rms_norm_q8(x, w, eps, residual, fmt, w_offset, normed, residual_out)
@@ -242,6 +246,72 @@ def w8a8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
     once (quantize_q8 lays its codes out so).  A bias that is not fp32 is
     converted in every call, by a launch of its own."""
     return _L.host().w8a8_linear(xq, xs, wq, ws, bias, out_dtype)
+
+
+# ----------------------------------------------------------------- e4m3 with a scale per block of 128, experts
+# Host side compiled and outputs without gradients, as above; expert_combine_grad and expert_combine are the gradients
+# of sorting tokens by expert and back, for a training loop to call.
+def quantize_f8(w):
+    """A weight [N, K], or [E, N, K] for experts, in e4m3 with a scale per 128 x
+    128 block: (float8_e4m3fn codes of its shape, fp32 scales [.., ceil(N/128),
+    ceil(K/128)] = max(amax, 1e-12) / 448).  Blocks at the ends may be smaller;
+    one with an infinity or a NaN gets the scale NaN and codes 0."""
+    return _L.host().quantize_f8(w)
+
+
+def f8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
+    """y[m, n] = sum_b (sum_{k in b} xq[m, k] * wq[n, k]) * xs[m, b] * ws[n // 128, b]
+    + bias[n] over the blocks b of 128 values of K: float8_e4m3fn activations
+    [M, K] with fp32 scales [M, ceil(K/128)] (fmt "e4m3_g128" above; of any
+    strides, but fastest as that lays them out), weights [N, K] with scales per
+    128 x 128 block (quantize_f8).  Blocks are summed in fp32.  Any M, N and K;
+    out_dtype bf16 or fp16, whose products are the matrix cores' fp8 ones (eight
+    at a time, cut to 2^-13 of the largest: 1.5e-5 of a result), or fp32, for
+    which they are exact, at half of the rate.  Code rows that do not start on 16 bytes are
+    copied first; a bias that is not fp32 is converted in every call."""
+    return _L.host().f8_linear(xq, xs, wq, ws, bias, out_dtype)
+
+
+def f8_linear_experts(xq, xs, wq, ws, offsets, tokens=None, out_dtype=torch.bfloat16):
+    """f8_linear over the rows of experts: rows offsets[e] .. offsets[e+1] - 1 of
+    the result are products with wq[e] and ws[e] (weights [E, N, K]).  With
+    tokens (int32 [P]), row s of the result [P, N] is that of row tokens[s] of xq
+    (the first product after expert_sort; nothing is gathered in memory);
+    without, of row s (the second).  offsets is int32 [E + 1], as expert_sort
+    gives it; rows from offsets[E] on are not written.  At most 4096 experts."""
+    return _L.host().f8_linear_experts(xq, xs, wq, ws, offsets, tokens, out_dtype)
+
+
+def expert_sort(ids, experts):
+    """The pairs (token, choice) of a router sorted by expert: ids int64 or int32
+    [T, k].  Returns int32 (offsets [experts + 1], tokens [T k], slots [T, k]):
+    expert e's rows are offsets[e] .. offsets[e+1] - 1, tokens[s] is the token of
+    row s, slots[t, j] the row of pair (t, j).  Rows of one expert keep the pairs'
+    order.  An id that is not in 0 .. experts - 1 (another rank's, a padded
+    token's) has slot -1 and no row; tokens behind the last row are -1."""
+    return _L.host().expert_sort(ids, experts)
+
+
+def expert_rows(x, tokens):
+    """x[tokens] [P, H] of rows x [T, H] of any type of 1, 2 or 4 bytes; rows whose
+    token is not in 0 .. T - 1 are zeros.  The gradient of x is
+    expert_combine(the rows' gradient, slots)."""
+    return _L.host().expert_rows(x, tokens)
+
+
+def expert_combine(y, slots, weights=None):
+    """out[t] = sum_j weights[t, j] * y[slots[t, j]] (ones without weights), summed
+    in fp32 in the order of j, in y's type.  y [P, H], slots int32 [T, k], weights
+    [T, k] bf16, fp16 or fp32.  Pairs whose slot is not in 0 .. P - 1 are left out."""
+    return _L.host().expert_combine(y, slots, weights)
+
+
+def expert_combine_grad(dout, y, slots, weights, tokens):
+    """The gradients (dy, dweights) of expert_combine for dout [T, H] of y's type:
+    dy[slots[t, j]] = weights[t, j] * dout[t] and zeros in rows without a token,
+    dweights[t, j] = dout[t] . y[slots[t, j]], 0 without a row.  tokens is
+    expert_sort's: no two slots are one row.  k <= 128, H <= 32768."""
+    return _L.host().expert_combine_grad(dout, y, slots, weights, tokens)
 
 
 def w8_linear_layers(x3, q3, s3, out_dtype=torch.bfloat16):
