@@ -332,7 +332,7 @@ int fp4x_f8_linear_experts(const void* xq, int64_t x_stride, const float* xs, in
                            const int* tokens, const int* offsets, int E, const void* wq, int64_t w_stride,
                            int64_t w_expert, const float* ws, void* out, int64_t out_stride, int out_dtype, int P,
                            int N, int K, void* stream);
-/* The forms (0 .. 10, from 16 x 16 to 256 x 256 tiles) that they take for a size
+/* The forms (0 .. 9, from 16 x 16 to 256 x 256 tiles) that they take for a size
  * on the current device; -1 for sizes below 1. */
 int fp4x_f8_form(int M, int N, int K, int out_dtype);
 int fp4x_f8_experts_form(int P, int N, int K, int E, int out_dtype);

@@ -25,6 +25,7 @@ struct F8Args {
   void* out;  int out_dtype;  int64_t out_stride;
   int M, N, K;
   int mt, nt, gm;                                  // tiles over M and N, tiles of M in a band
+  int stream;                                      // large tiles: the output passes by the L2
   // experts
   const int *offsets, *tokens;                     // [E + 1]; rows of x or null
   int E, X;                                        // X: rows of x
@@ -47,15 +48,19 @@ __device__ __forceinline__ int wave_sum_to(int v) {
   return v;
 }
 
-// The tile of workgroup `id` among the experts' tiles: expert by expert, a band
-// of its rows' tiles per BN columns.  Every wave finds it by itself: a lane sums
-// the tiles of E / 64 experts, one scan gives the total and the lane that holds
-// the tile, and a second one the expert.  Offsets that do not rise, or leave the
-// output's rows, give empty experts.  False: no tile is left for this workgroup.
+// A workgroup's tiles among the experts': expert by expert, the tiles of its rows
+// per BN columns.  An XCD takes a run of consecutive tiles, in rounds of one per
+// workgroup; a round is dealt one workgroup on from the round before, so that an
+// expert's last tiles, which may hold a few rows only, do not all fall to some.
+// Every wave finds them by itself: a lane sums the tiles of E / 64 experts, a scan
+// gives the total, and then lane j looks its workgroup's tile j up, among the
+// lanes' sums and then among the experts of one lane.  Offsets that do not rise,
+// or leave the output's rows, give empty experts.  Returns the number of tiles,
+// which the grid keeps to 64 at most; lane j < that holds tile j's place.
 template <int BM, int BN>
-__device__ __forceinline__ bool f8_expert_tile(const F8Args& a, int id, F8Place& p) {
+__device__ __forceinline__ int f8_expert_tiles(const F8Args& a, F8Place& p) {
   const int lane = threadIdx.x & 63, per = (a.E + 63) >> 6;
-  const auto at = [&](int e) { return min(max(a.offsets[min(e, a.E)], 0), a.M); };
+  const auto at = [&](int e) __attribute__((always_inline)) { return min(max(a.offsets[min(e, a.E)], 0), a.M); };
   int sum = 0;
   for (int b = 0; b < per; b += 8) {
     int o[9];
@@ -64,22 +69,72 @@ __device__ __forceinline__ bool f8_expert_tile(const F8Args& a, int id, F8Place&
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += (max(o[i + 1] - o[i], 0) + BM - 1) / BM;
   }
-  const int upto = wave_sum_to(sum), total = __builtin_amdgcn_readlane(upto, 63);
-  const I8Run run(total * a.nt, id & 7);
-  if ((id >> 3) >= run.count) return false;
-  const int t = run.first + (id >> 3), mt = t / a.nt;     // mt: the tile's place if every expert had one column
-  const int l = __builtin_ctzll(__ballot(upto > mt));
-  const int before = __builtin_amdgcn_readlane(upto - sum, l);
+  const int upto = wave_sum_to(sum), hit = min(a.M, a.E);   // (rising offsets stay within the bound by themselves)
+  const int total = min(__builtin_amdgcn_readlane(upto, 63), (a.M - hit) / BM + hit) * a.nt;
+  const int xcd = blockIdx.x & 7, stride = (gridDim.x + 7 - xcd) >> 3, own = blockIdx.x >> 3;
+  const I8Run run(total, xcd);
+  const int rounds = run.count / stride, rest = run.count - rounds * stride;
+  const int tiles = rounds + ((own + rounds) % stride < rest);
+  const int t = run.first + min(lane * stride + (own + lane) % stride, max(run.count - 1, 0));
+  const int mt = t / a.nt;                         // the tile's place if every expert had one column
+  int l = 0;
+#pragma unroll
+  for (int h = 32; h; h >>= 1)
+    if (__shfl(upto, l + h - 1) <= mt) l += h;
+  int begin = __shfl(upto - sum, l), found = 0, many = 1;
+  p = F8Place{0, 0, 0, 0};
+  for (int b = 0; b < per; b += 8) {
+    int o[9];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) o[i] = at(l * per + min(b + i, per));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int n = (max(o[i + 1] - o[i], 0) + BM - 1) / BM;
+      if (mt >= begin && mt < begin + n) {
+        p.e = l * per + b + i;
+        p.m0 = o[i];
+        p.m_end = o[i + 1];
+        found = begin;
+        many = n;
+      }
+      begin += n;
+    }
+  }
+  const int r = t - found * a.nt, n = r / many;
+  p.m0 += (r - n * many) * BM;
+  p.n0 = n * BN;
+  return tiles;
+}
+// The same for one tile per workgroup, which the lanes look up together: the second time each takes an expert (24 rows of
+// 512 experts took 18.1 us with the function above, 17.0 with this).
+template <int BM, int BN>
+__device__ __forceinline__ bool f8_expert_tile(const F8Args& a, F8Place& p) {
+  const int lane = threadIdx.x & 63, per = (a.E + 63) >> 6;
+  const auto at = [&](int e) __attribute__((always_inline)) { return min(max(a.offsets[min(e, a.E)], 0), a.M); };
+  int sum = 0;
+  for (int b = 0; b < per; b += 8) {
+    int o[9];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) o[i] = at(lane * per + min(b + i, per));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += (max(o[i + 1] - o[i], 0) + BM - 1) / BM;
+  }
+  const int upto = wave_sum_to(sum);
+  const I8Run run(__builtin_amdgcn_readlane(upto, 63) * a.nt, blockIdx.x & 7);
+  if ((int)(blockIdx.x >> 3) >= run.count) return false;
+  const int t = run.first + (blockIdx.x >> 3), mt = t / a.nt;
+  const int l = __builtin_ctzll(__ballot(upto > mt)), before = __builtin_amdgcn_readlane(upto - sum, l);
   const int e = l * per + min(lane, per), lo = at(e), hi = at(lane < per ? e + 1 : e);
   const int tiles = (max(hi - lo, 0) + BM - 1) / BM, to = before + wave_sum_to(tiles);
   const int i = __builtin_ctzll(__ballot(to > mt));
   const int own = __builtin_amdgcn_readlane(tiles, i), first = __builtin_amdgcn_readlane(to, i) - own;
   const int r = t - first * a.nt, n = own == 1 ? r : r / own;
-  p.e = l * per + i;
-  p.m0 = __builtin_amdgcn_readlane(lo, i) + (r - n * own) * BM;
-  p.m_end = __builtin_amdgcn_readlane(hi, i);
-  p.n0 = n * BN;
+  p = F8Place{__builtin_amdgcn_readlane(lo, i) + (r - n * own) * BM, __builtin_amdgcn_readlane(hi, i), n * BN, l * per + i};
   return true;
+}
+__device__ __forceinline__ F8Place f8_place_of(const F8Place& p, int j) {   // lane j's, for all
+  return F8Place{__builtin_amdgcn_readlane(p.m0, j), __builtin_amdgcn_readlane(p.m_end, j), __builtin_amdgcn_readlane(p.n0, j),
+                 __builtin_amdgcn_readlane(p.e, j)};
 }
 
 // Direct load of 4 bytes per lane, each from an address of its own, to lds + 4 lane.
@@ -138,6 +193,14 @@ __device__ __forceinline__ void f8_store4(const F8Args& a, int64_t m, int n, con
   }
 }
 
+// 16 bytes of the output.  One that is larger than the 32 MB of the XCDs' L2 passes by it: it would push out the rows of x
+// and w that the next tiles share (4096 x [16384 x 2560] took 175 us so, 163 with these stores).
+template <class V>
+__device__ __forceinline__ void f8_put(V* at, V v, int stream) {
+  if (stream) asm volatile("global_store_dwordx4 %0, %1, off nt" ::"v"(at), "v"(v) : "memory");   // (two plain stores would be merged)
+  else *at = v;
+}
+
 // ------------------------------------------------------------------ small tiles
 // A workgroup owns 16 MT rows of x and 16 NT rows of w; its W waves split K in
 // units of 128 values, a block of scales each, and bring them through rings of
@@ -155,7 +218,7 @@ __global__ __launch_bounds__(64 * W, 2) void f8_ring_kernel(const F8Args a) {
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 15, g = lane >> 4;
   F8Place p{0, a.M, 0, 0};
   if constexpr (EX) {
-    if (!f8_expert_tile<16 * MT, 16 * NT>(a, blockIdx.x, p)) return;
+    if (!f8_expert_tile<16 * MT, 16 * NT>(a, p)) return;
   } else {
     const I8Run run(a.mt * a.nt, blockIdx.x & 7);
     tile_place(a.mt, a.nt, a.gm, run.first + (blockIdx.x >> 3), 16 * MT, 16 * NT, p.m0, p.n0);
@@ -307,10 +370,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
   constexpr int MS = C::MS, NS = C::NS, NL = C::NL;
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  F8Place p{0, a.M, 0, 0};
+  F8Place all;                                     // EX: lane j holds tile j's
   int first = 0, stride = 1, tiles = 1;
   if constexpr (EX) {
-    if (!f8_expert_tile<BM, BN>(a, blockIdx.x, p)) return;
+    tiles = f8_expert_tiles<BM, BN>(a, all);
+    if (tiles < 1) return;
   } else {
     const int xcd = blockIdx.x & 7;
     const I8Run run(a.mt * a.nt, xcd);
@@ -323,62 +387,84 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
   const bool tail = a.K & 127;                     // K ends inside a k-tile
   const bool pick = EX && a.tokens;
 
+  // The lane, where what is computed from it is not to be kept in registers through the loop over K (the 256 x 256 tiles
+  // have none left; a value that is spilled there is loaded again behind a wait for every load on its way).
+  const auto lane_here = [&]() __attribute__((always_inline)) {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+
   // ---- the loads: k-tile lk of tile lt
   // LDS row r holds chunk c of its 128 bytes at c ^ key: the 16 lanes that LDS serves together read different banks
-  const int slot = lane & 7, lr = lane >> 3;
   const uint32_t lbase = i8_lds(lds);
-  int lt = 0, lk = 0, lm0 = p.m0, ln0 = p.n0;
+  int lt = 0, lk = 0;
+  F8Place lp{0, a.M, 0, 0};
   int pm0 = 0, pn0 = 0, pm1 = 0, pn1 = 0;          // places of an even and of an odd tile
   uint32_t off[NL - 1];
   const uint8_t *xb, *wb;
-  const float* sp;                                 // the scale that this lane brings of each k-tile
+  uint32_t soff;                                   // the scale that this lane brings of each k-tile
+  const float* sb;
   const int64_t sstep = wave < BM / 64 ? a.sx_b : 1;
-  const auto row_of = [&](int j) __attribute__((always_inline)) {   // LDS row of load j in its operand's half
-    return ((j < C::XL ? wave * C::XL + j : wave * C::WL + j - C::XL) << 3) + lr;
+  const auto row_of = [&](int j, int l) __attribute__((always_inline)) {   // LDS row of load j in its operand's half
+    return ((j < C::XL ? wave * C::XL + j : wave * C::WL + j - C::XL) << 3) + (l >> 3);
   };
   const auto x_row = [&](int r) __attribute__((always_inline)) {    // row of x of row r of the tile
-    const int m = min(lm0 + r, p.m_end - 1);
+    const int m = min(lp.m0 + r, lp.m_end - 1);
     return pick ? min(max(a.tokens[m], 0), a.X - 1) : m;
   };
   const auto next_tile = [&]() __attribute__((always_inline)) {
-    if constexpr (!EX) tile_place(a.mt, a.nt, a.gm, first + lt * stride, BM, BN, lm0, ln0);
-    if (lt & 1) {
-      pm1 = lm0;
-      pn1 = ln0;
+    if constexpr (EX) {
+      lp = f8_place_of(all, lt);
     } else {
-      pm0 = lm0;
-      pn0 = ln0;
-    }
-#pragma unroll
-    for (int j = 0; j < NL - 1; ++j) {
-      const int r = row_of(j), c = slot ^ ((r >> 1) & 7);
-      if (j < C::XL) off[j] = (uint32_t)(x_row(r) - (pick ? 0 : lm0)) * (uint32_t)a.x_stride + c * 16;
-      else {
-        const int wr = (r & -(16 * NS)) + ((r & 15) >> 2) * (4 * NS) + ((r >> 4) % NS) * 4 + (r & 3);
-        off[j] = (uint32_t)(min(ln0 + wr, a.N - 1) - ln0) * (uint32_t)a.w_stride + c * 16;
+      tile_place(a.mt, a.nt, a.gm, first + lt * stride, BM, BN, lp.m0, lp.n0);
+      if (lt & 1) {
+        pm1 = lp.m0;
+        pn1 = lp.n0;
+      } else {
+        pm0 = lp.m0;
+        pn0 = lp.n0;
       }
     }
-    xb = a.x + (pick ? 0 : lm0 * a.x_stride);
-    wb = a.w + p.e * a.w_estride + ln0 * a.w_stride;
+    const int l = lane_here();
+#pragma unroll
+    for (int j = 0; j < NL - 1; ++j) {
+      const int r = row_of(j, l), c = (l & 7) ^ ((r >> 1) & 7);
+      if (j < C::XL) off[j] = (uint32_t)(x_row(r) - (pick ? 0 : lp.m0)) * (uint32_t)a.x_stride + c * 16;
+      else {
+        const int wr = (r & -(16 * NS)) + ((r & 15) >> 2) * (4 * NS) + ((r >> 4) % NS) * 4 + (r & 3);
+        off[j] = (uint32_t)(min(lp.n0 + wr, a.N - 1) - lp.n0) * (uint32_t)a.w_stride + c * 16;
+      }
+    }
+    xb = a.x + (pick ? 0 : lp.m0 * a.x_stride);
+    wb = a.w + lp.e * a.w_estride + lp.n0 * a.w_stride;
     const int nbs = (a.N + 127) >> 7;
-    sp = wave < BM / 64 ? a.sx + x_row(wave * 64 + lane) * a.sx_m
-                        : a.sw + ((int64_t)p.e * nbs + min((ln0 >> 7) + lane, nbs - 1)) * kts;
+    if (wave < BM / 64) {
+      soff = (uint32_t)(x_row(wave * 64 + l) - (pick ? 0 : lp.m0)) * (uint32_t)a.sx_m * 4;
+      sb = a.sx + (pick ? 0 : lp.m0 * a.sx_m);
+    } else {                                       // (several waves bring the same values)
+      soff = min(l, nbs - 1 - (lp.n0 >> 7)) * kts * 4;
+      sb = a.sw + ((int64_t)lp.e * nbs + (lp.n0 >> 7)) * kts;
+    }
     // its bias, before its first k-tile, so it is there when that is
     if (!EX && a.bias)
       for (int e = wave; e < BN / 64; e += C::W)
-        i8_load4(lbase + S * C::STAGE + (lt & 1) * BN * 4 + e * 256, min(ln0 + e * 64 + lane, a.N - 1) * 4, a.bias);
+        i8_load4(__builtin_amdgcn_readfirstlane(lbase + S * C::STAGE + (lt & 1) * BN * 4 + e * 256), min(lp.n0 + e * 64 + l, a.N - 1) * 4, a.bias);
   };
   const auto clamp_tail = [&]() __attribute__((always_inline)) {   // chunks past a row's last one read that one
+    const int l = lane_here();
 #pragma unroll
     for (int j = 0; j < NL - 1; ++j) {
-      const int over = lk * 8 + (slot ^ ((row_of(j) >> 1) & 7)) - last;
+      const int over = lk * 8 + ((l & 7) ^ ((row_of(j, l) >> 1) & 7)) - last;
       if (over > 0) off[j] -= over * 16;
     }
   };
   const auto load = [&](int j, int so) __attribute__((always_inline)) {
-    if (j < C::XL) i8_load16(lbase + so + (wave * C::XL + j) * 1024, off[j], xb + lk * 128);
-    else if (j < NL - 1) i8_load16(lbase + so + BM * 128 + (wave * C::WL + j - C::XL) * 1024, off[j], wb + lk * 128);
-    else f8_load4(lbase + so + (BM + BN) * 128 + (wave < BM / 64 ? wave : BM / 64) * 256, sp + lk * sstep);   // (w's: several waves, one value)
+    const auto to = [&](int at) { return __builtin_amdgcn_readfirstlane(lbase + so + at); };   // (scalars, for the asm)
+    const int k = __builtin_amdgcn_readfirstlane(lk);
+    if (j < C::XL) i8_load16(to((wave * C::XL + j) * 1024), off[j], xb + k * 128);
+    else if (j < NL - 1) i8_load16(to(BM * 128 + (wave * C::WL + j - C::XL) * 1024), off[j], wb + k * 128);
+    else i8_load4(to((BM + BN) * 128 + min(wave, BM / 64) * 256), soff, sb + k * sstep);
   };
   const auto advance = [&]() __attribute__((always_inline)) {
     if (++lk == kts) {
@@ -391,7 +477,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
   // Zeros in place of what lies past K in a tile's last k-tile: both operands', since those bytes may be NaN codes.
   // (In LDS, behind a barrier of its own: masks in registers would not fit beside 256 x 256 sums.)
   const auto cut = [&](int so) __attribute__((always_inline)) {
-    for (int r = t; r < BM + BN; r += 64 * C::W)
+    for (int r = wave * 64 + lane_here(); r < BM + BN; r += 64 * C::W)
       for (int c = (a.K & 127) >> 4; c < 8; ++c) {
         i32x4_t* at = reinterpret_cast<i32x4_t*>(lds + so + r * 128 + ((c ^ ((r >> 1) & 7)) * 16));
         *at = keep_to(*at, c, a.K & 127);
@@ -401,12 +487,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
 
   // ---- the products
   const int wm = wave % WM, wn = wave / WM, i = lane & 15, g = lane >> 4, key = (i >> 1) & 7;
-  const int xrow = wm * 16 * MS + i, wrow = BM + wn * 16 * NS + i, c0 = (g ^ key) * 16, c1 = ((4 + g) ^ key) * 16;
-  const int sx_at = (BM + BN) * 128 + xrow * 4, sw_at = (BM + BN) * 128 + BM * 4 + (wn * 16 * NS / 128) * 4;
+  // a lane's chunks of the first strip of x, and how far on the first one of w is
+  const int c0 = (wm * 16 * MS + i) * 128 + (g ^ key) * 16, c1 = (wm * 16 * MS + i) * 128 + ((4 + g) ^ key) * 16;
+  const int w_on = (BM + wn * 16 * NS - wm * 16 * MS) * 128;
+  const int sx_at = (BM + BN) * 128 + (wm * 16 * MS + i) * 4, sw_at = (BM + BN) * 128 + BM * 4 + (wn * 16 * NS / 128) * 4;
   f32x4_t acc[MS][NS], part[4];
   i32x8_t x[2], w[NS];
   F8Frag<B16> wf[NS];
-  float f[2], sw = 0.0f, sx_next = 0.0f, sw_next = 0.0f;   // f: both scales of a strip
+  float f[2], sx, sw;                              // f: both scales of a strip, of the next one still apart
   const auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < MS; ++s)
@@ -415,31 +503,45 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
     part[2] = part[3] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};   // nothing waits to be added
     f[1] = 0.0f;
   };
-  const auto fetch = [&](int so, int row) __attribute__((always_inline)) {
-    const char* at = lds + so + row * 128;
-    return f8_cat(*reinterpret_cast<const i32x4_t*>(at + c0), *reinterpret_cast<const i32x4_t*>(at + c1));
+  const auto fetch = [&](int so, int strip) __attribute__((always_inline)) {   // of x; of w: so + w_on
+    return f8_cat(*reinterpret_cast<const i32x4_t*>(lds + so + c0 + strip * 2048),
+                  *reinterpret_cast<const i32x4_t*>(lds + so + c1 + strip * 2048));
   };
   const auto scale = [&](int so, int s) __attribute__((always_inline)) {
     return *reinterpret_cast<const float*>(lds + so + sx_at + 64 * s);
   };
-  int ek = 0;                                      // the k-tile that is multiplied
+  int ek = 0, et = 0;                              // the k-tile that is multiplied, and its tile
+  bool busy = true;                                // EX: whether the tile has rows for this wave
+  const auto look = [&]() __attribute__((always_inline)) {
+    if constexpr (EX) {
+      const F8Place ep = f8_place_of(all, min(et, tiles - 1));
+      busy = ep.m0 + wm * 16 * MS < ep.m_end;
+    }
+  };
   const auto add = [&](int e) __attribute__((always_inline)) {   // block e of a k-tile into its sums
     const int s = e / NS, r = e % NS;
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[s][r][j] = __builtin_fmaf(part[e & 3][j], f[s & 1], acc[s][r][j]);
     asm volatile("" : "+v"(acc[s][r]));            // here, not sunk to a later block with its part kept until then
   };
+  const auto first_of = [&](int so) __attribute__((always_inline)) {   // a k-tile's first reads
+#pragma unroll
+    for (int r = 0; r < NS; ++r) w[r] = fetch(so + w_on, r);
+    x[0] = fetch(so, 0);
+    sx = scale(so, 0);
+    sw = *reinterpret_cast<const float*>(lds + so + sw_at);
+  };
   // Step s of a k-tile in stage so.  In the last step `more` reads from the next stage `nx`, and `fill` issues the loads
-  // of the stage that the barrier freed.
+  // of the stage that the barrier freed.  The order is pinned: an MFMA, then what does not wait for it.
+  // A wave that the tile has no rows for only takes its part in the loads.
   const auto step = [&](int s, int so, bool more, int nx, bool fill) __attribute__((always_inline)) {
     const bool end = s == MS - 1;
-    if (!end) {
-      x[(s + 1) & 1] = fetch(so, xrow + 16 * (s + 1));
-      sx_next = scale(so, s + 1);
-    } else if (more) {
-      x[0] = fetch(nx, xrow);
-      sx_next = scale(nx, 0);
-      sw_next = *reinterpret_cast<const float*>(lds + nx + sw_at);
+    if (EX && !busy) {
+      if (fill)
+#pragma unroll
+        for (int j = 0; j < NL; ++j) load(j, so);
+      if (end && more) first_of(nx);
+      return;
     }
     F8Frag<B16> xf;
     xf.set(x[s & 1]);
@@ -449,73 +551,121 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
       const int e = s * NS + r;
       if (!B16 || s == 0) wf[r].set(w[r]);
       part[e & 3] = f8_block(wf[r], xf);
-      if (end && more) w[r] = fetch(nx, wrow + 16 * r);
+      if (!end) __builtin_amdgcn_sched_barrier(0);
+      if (r == 0 && !end) x[(s + 1) & 1] = fetch(so, s + 1);
+      if (r == 0 && end && more) x[0] = fetch(nx, 0);
+      if (end && more) w[r] = fetch(nx + w_on, r);
       add(e < 2 ? e - 2 + MS * NS : e - 2);
+      if (r == 1) {                                // the strip before is done with its scales
+        f[s & 1] = sx * sw;
+        if (!end) sx = scale(so, s + 1);
+        if (end && more) {
+          sx = scale(nx, 0);
+          sw = *reinterpret_cast<const float*>(lds + nx + sw_at);
+        }
+      }
       if (fill)
         while (j < NL && (r == NS - 1 || j * NS <= r * NL)) load(j++, so);
-      __builtin_amdgcn_sched_barrier(0);           // this order of loads, reads and MFMAs
+      if (!end) {
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        __builtin_amdgcn_sched_group_barrier(0x008, B16 ? 4 : 1, 0);
+        if (more) {
+          if (r < 2) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+          else __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        if (r == 1) __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+        else __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
     }
-    if (end) sw = sw_next;
-    f[(s + 1) & 1] = sx_next * sw;                 // (the blocks that wait are of this step)
   };
 
   // ---- a tile's end
-  int et = 0, drain = 0;
-  const auto put = [&](auto dt, bool full, int em0, int n, const float (&bs)[4 * NS]) __attribute__((always_inline)) {
-    constexpr int DT = decltype(dt)::value;
+  int drain = 0;
+  // A lane's 4 NS columns of a row are NP pieces of 16 bytes.  The four lanes of a row exchange theirs (rows of 16 lanes,
+  // then halves of the wave), so that a store would write 64 bytes of each of 16 rows, and then the halves of 8 rows: a
+  // store writes whole lines of 8 rows (NP 1: 64 bytes of 16).
+  const auto put = [&](auto dt, int l, const F8Place& ep, int n0, const float (&bs)[4 * NS]) __attribute__((always_inline)) {
+    constexpr int DT = decltype(dt)::value, PER = DT == DT_F32 ? 4 : 8, NP = 4 * NS / PER;
 #pragma unroll
     for (int s = 0; s < MS; ++s) {
-      const int m = em0 + wm * 16 * MS + 16 * s + i;
-      const int64_t at = m * a.out_stride + n;
-      float v[4 * NS];
+      uint32_t d[NP][4];
 #pragma unroll
-      for (int q = 0; q < 4 * NS; ++q) v[q] = acc[s][q >> 2][q & 3] + bs[q];
-      if (!full) {
-        if (m < p.m_end)
+      for (int q = 0; q < NP; ++q)
 #pragma unroll
-          for (int q = 0; q < 4 * NS; ++q)
-            if (n + q < a.N) store_out(a.out, at + q, DT, v[q]);
-      } else if constexpr (DT == DT_F32) {
-        if (!EX || m < p.m_end)
-#pragma unroll
-          for (int q = 0; q < NS; ++q)
-            *reinterpret_cast<u32x4_a4*>(static_cast<float*>(a.out) + at + 4 * q) =
-                u32x4_a4{__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
-                         __float_as_uint(v[4 * q + 3])};
-      } else {
-        if (!EX || m < p.m_end)
-#pragma unroll
-          for (int q = 0; q < NS / 2; ++q) {
-            uint32_t d[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              d[k] = DT == DT_BF16 ? pack_bf16x2(v[8 * q + 2 * k], v[8 * q + 2 * k + 1])
-                                   : pack_f16x2(v[8 * q + 2 * k], v[8 * q + 2 * k + 1]);
-            *reinterpret_cast<u32x4_a2*>(static_cast<uint16_t*>(a.out) + at + 8 * q) = u32x4_a2{d[0], d[1], d[2], d[3]};
+        for (int k = 0; k < 4; ++k) {
+          const int c = PER * q + PER / 4 * k;
+          const float lo = acc[s][c >> 2][c & 3] + bs[c];
+          if constexpr (DT == DT_F32) {
+            d[q][k] = __float_as_uint(lo);
+          } else {
+            const float hi = acc[s][c >> 2][(c & 3) + 1] + bs[c + 1];
+            d[q][k] = DT == DT_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
           }
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int q = 0; q + 1 < NP; q += 2) {
+          const auto v = __builtin_amdgcn_permlane16_swap(d[q][k], d[q + 1][k], false, false);
+          d[q][k] = v[0];
+          d[q + 1][k] = v[1];
+        }
+#pragma unroll
+        for (int q = 0; q < NP / 2; ++q) {
+          const auto v = __builtin_amdgcn_permlane32_swap(d[q][k], d[q + NP / 2][k], false, false);
+          d[q][k] = v[0];
+          d[q + NP / 2][k] = v[1];
+        }
+#pragma unroll
+        for (int q = 0; q + 1 < NP; q += 2) {      // lanes 8 to 15 of 16 <-> lanes 0 to 7, of the other piece
+          const int u = (int)d[q][k], v = (int)d[q + 1][k];
+          d[q][k] = (uint32_t)__builtin_amdgcn_update_dpp(u, v, 0x128, 0xf, 0xc, false);
+          d[q + 1][k] = (uint32_t)__builtin_amdgcn_update_dpp(v, u, 0x128, 0xf, 0x3, false);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        const int row = NP == 1 ? l & 15 : 8 * (q & 1) + (l & 7), piece = NP == 1 ? l >> 4 : 8 * (q >> 1) + (l >> 1 & 4) + (l >> 4);
+        const int m = ep.m0 + wm * 16 * MS + 16 * s + row, n = n0 + piece * PER;
+        if (m < ep.m_end) {
+          const int64_t at = m * a.out_stride + n;
+          if (n + PER > a.N) {
+            for (int k = 0; k < PER && n + k < a.N; ++k) {
+              if constexpr (DT == DT_F32) static_cast<uint32_t*>(a.out)[at + k] = k < 2 ? (k ? d[q][1] : d[q][0]) : d[q][2];
+              else static_cast<uint16_t*>(a.out)[at + k] = (uint16_t)((k < 2 ? d[q][0] : k < 4 ? d[q][1] : k < 6 ? d[q][2] : d[q][3]) >> (16 * (k & 1)));
+            }
+          } else if constexpr (DT == DT_F32) {
+            f8_put(reinterpret_cast<u32x4_a4*>(static_cast<float*>(a.out) + at), u32x4_a4{d[q][0], d[q][1], d[q][2], d[q][3]}, a.stream);
+          } else {
+            f8_put(reinterpret_cast<u32x4_a2*>(static_cast<uint16_t*>(a.out) + at), u32x4_a2{d[q][0], d[q][1], d[q][2], d[q][3]}, a.stream);
+          }
+        }
       }
     }
   };
   const auto finish = [&]() __attribute__((always_inline)) {
+    if (EX && !busy) {
+      drain = 0;
+      ++et;
+      return;
+    }
     add(MS * NS - 2);
     add(MS * NS - 1);
     asm volatile("" ::: "memory");                 // the stores come after the loads of this k-tile
-    const int em0 = et & 1 ? pm1 : pm0, en0 = et & 1 ? pn1 : pn0;
+    F8Place ep{et & 1 ? pm1 : pm0, a.M, et & 1 ? pn1 : pn0, 0};
+    if constexpr (EX) ep = f8_place_of(all, et);
     const float* bp = reinterpret_cast<const float*>(lds + S * C::STAGE + (et & 1) * BN * 4);
-    const int nl = wn * 16 * NS + 4 * NS * g, n = en0 + nl;
-    float bs[4 * NS];
+    const int l = lane_here(), nl = wn * 16 * NS, n0 = ep.n0 + nl;
+    float bs[4 * NS] = {};
+    if (!EX && a.bias)
 #pragma unroll
-    for (int q = 0; q < 4 * NS; ++q) bs[q] = !EX && a.bias ? bp[nl + q] : 0.0f;
-    const bool full = (EX || em0 + BM <= a.M) && en0 + BN <= a.N;
-    const auto go = [&](auto dt) __attribute__((always_inline)) {
-      if (full) put(dt, true, em0, n, bs);
-      else put(dt, false, em0, n, bs);
-    };
-    if constexpr (B16) go(std::integral_constant<int, DT_F32>());
-    else if (a.out_dtype == DT_BF16) go(std::integral_constant<int, DT_BF16>());
-    else go(std::integral_constant<int, DT_F16>());
+      for (int q = 0; q < 4 * NS; ++q) bs[q] = bp[nl + 4 * NS * (l >> 4) + q];
+    if constexpr (B16) put(std::integral_constant<int, DT_F32>(), l, ep, n0, bs);
+    else if (a.out_dtype == DT_BF16) put(std::integral_constant<int, DT_BF16>(), l, ep, n0, bs);
+    else put(std::integral_constant<int, DT_F16>(), l, ep, n0, bs);
     // at least MS NS / 2 stores, all newer than the loads of the next S - 1 k-tiles (a tile that ends at M or N may store less)
-    drain = full ? S - 1 : 0;
+    drain = ep.m0 + BM <= ep.m_end && ep.n0 + BN <= a.N ? S - 1 : 0;
     ++et;
     asm volatile("" ::: "memory");
   };
@@ -533,11 +683,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
   else i8_sync<0>();
   if (tail && kts == 1) cut(0);
   clear();
-#pragma unroll
-  for (int r = 0; r < NS; ++r) w[r] = fetch(0, wrow + 16 * r);
-  x[0] = fetch(0, xrow);
-  sw = *reinterpret_cast<const float*>(lds + sw_at);
-  f[0] = scale(0, 0) * sw;
+  look();
+  first_of(0);
 #pragma unroll
   for (int s = 0; s < MS - 1; ++s) step(s, 0, true, 0, false);
   int so = 0, v = 0;
@@ -555,6 +702,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
     if (++ek == kts) {
       finish();
       clear();
+      look();
       ek = 0;
     }
 #pragma unroll
@@ -570,6 +718,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
     if (++ek == kts) {
       finish();
       clear();
+      look();
       ek = 0;
     }
 #pragma unroll
@@ -585,6 +734,12 @@ void launch_f8_tile(dim3 grid, const F8Args& a, hipStream_t st) {
   const dim3 threads(64 * WM * WN);
   hipLaunchKernelGGL((f8_tile_kernel<BM, BN, WM, WN, S, EX, B16>), grid, threads, 0, st, a);
 }
+
+// The forms: 0 to 3 small tiles, 4 to 9 large ones; and which of them there are, plain and over experts, for 16-bit and (B16)
+// fp32 outputs.  One is left out where the others cost less than 1% more without it (the sizes are fp4x_f8.hip's); 256 x 256
+// tiles have no room for bf16 operands beside their sums.
+constexpr int kF8Forms = 10;
+constexpr uint32_t kF8Have[2][2] = {{0x3ff, 0x0b7}, {0x2b6, 0x0b6}};   // [experts][B16], bit f: form f
 
 // The launch of each form (fp4x_f8_forms.h), in units of their own.
 void launch_f8_dense(int form, dim3 grid, const F8Args& a, hipStream_t st);

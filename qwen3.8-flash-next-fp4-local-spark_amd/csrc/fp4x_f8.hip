@@ -1,5 +1,6 @@
 // f8_linear and f8_linear_experts: which form a size takes, its launch and the C
 // entry points (kernels: fp4x_f8.h).
+#include <cmath>
 #include <string>
 
 #include "fp4x_f8.h"
@@ -12,25 +13,41 @@ int device_cus();
 // ------------------------------------------------------------------ choice
 constexpr int64_t kF8MaxStride = (1 << 24) - 16;   // 256 rows within 32-bit offsets
 
-struct F8Form { int bm, bn, slots, ring, stages; float a, b, d; };
-constexpr F8Form kF8Forms[] = {
-    {16, 16, 2, 1, 2, 2.14f, 0.53f, 0.028f}, {16, 32, 2, 1, 3, 2.13f, 0.57f, 0.061f},
-    {16, 64, 2, 1, 2, 2.26f, 0.62f, 0.111f}, {32, 32, 2, 1, 2, 2.18f, 0.59f, 0.076f},
-    {32, 64, 1, 1, 2, 1.32f, 2.20f, 0.144f}, {64, 64, 2, 0, 4, 2.67f, 0.77f, 0.276f},
-    {64, 128, 2, 0, 3, 2.93f, 1.12f, 0.312f}, {128, 128, 1, 0, 4, 0.89f, 2.80f, 0.519f},
-    {128, 128, 2, 0, 2, 3.00f, 1.72f, 0.583f}, {256, 128, 1, 0, 3, 2.43f, 4.24f, 0.855f},
-    {256, 256, 1, 0, 2, 5.83f, 5.42f, 1.341f}};
-constexpr int kF8Count = sizeof(kF8Forms) / sizeof(kF8Forms[0]);
+struct F8Form { int bm, bn, slots, ring, stages; };
+constexpr F8Form kF8Shape[kF8Forms] = {{16, 16, 2, 1, 2},   {16, 32, 2, 1, 3},   {32, 32, 2, 1, 2},   {32, 64, 1, 1, 2},
+                                       {64, 64, 2, 0, 4},   {64, 128, 2, 0, 3},  {128, 128, 1, 0, 4}, {128, 128, 2, 0, 2},
+                                       {256, 128, 1, 0, 3}, {256, 256, 1, 0, 2}};
 
-static int f8_best(int K, bool b16, int64_t (*tiles)(const F8Form&, int64_t, int64_t, int64_t), int64_t M, int64_t N, int64_t E) {
-  const int cus = device_cus();
-  const float k = (float)((K + 127) / 128);
-  int best = 0;
+// Forms are ranked by a + n (b + d k): n tiles fall to a CU, each with k = ceil(K / 128) k-tiles, and the one with the least
+// is taken.  a, b and d are fitted to 1,000 sizes (1 to 8192 rows, 16 to 18000 columns, K from 64 to 10240; 1 to 512 experts;
+// most drawn evenly over their logarithms, weights from HBM; profiles/f8_forms.txt), so that the form taken is near the
+// fastest: on average 0.5% slower (products, 16-bit outputs; 11% at most), 0.8% (fp32 outputs; 22%), 1.3% and 1.1% (over
+// experts; 23% and 14%).  Their sums are no times: only their order counts.
+struct F8Cost { float a, b, d; };
+constexpr F8Cost kF8Cost[2][2][kF8Forms] = {
+    {{{0.84f, 0.852f, 0.0396f}, {1.12f, 0.858f, 0.0582f}, {1.28f, 1.022f, 0.0661f}, {0.80f, 3.811f, 0.0805f},
+      {2.28f, 1.213f, 0.2582f}, {4.64f, 1.748f, 0.2608f}, {0.34f, 6.016f, 0.3885f}, {9.13f, 0.812f, 0.3704f},
+      {0.00f, 7.808f, 0.6867f}, {0.00f, 13.045f, 1.0335f}},
+     {{0.91f, 1.241f, 0.0302f}, {1.23f, 1.373f, 0.0429f}, {1.32f, 1.652f, 0.0484f}, {}, {3.95f, 0.340f, 0.7088f},
+      {5.22f, 2.532f, 0.4773f}, {}, {0.41f, 8.166f, 0.6476f}, {}, {}}},
+    {{{}, {0.56f, 1.944f, 0.0740f}, {1.24f, 1.698f, 0.1402f}, {}, {4.23f, 0.710f, 0.3542f}, {4.51f, 0.720f, 0.4488f}, {},
+      {5.20f, 0.951f, 0.5319f}, {}, {11.47f, 3.946f, 1.0354f}},
+     {{}, {0.64f, 3.149f, 0.0408f}, {1.37f, 3.270f, 0.0583f}, {}, {6.15f, 0.601f, 1.1460f}, {11.16f, 0.760f, 0.5155f}, {},
+      {12.76f, 1.004f, 0.6093f}, {}, {}}}};
+
+// rows of tiles: for a form's height, how many.
+template <class Rows>
+static int f8_best(int ex, bool b16, int N, int K, Rows rows) {
+  const float k = (float)((K + 127) / 128), cus = (float)device_cus();
+  int best = -1;
   float least = 0.0f;
-  for (int f = 0; f < kF8Count - b16; ++f) {     // (the last form has no bf16 products)
-    const F8Form& c = kF8Forms[f];
-    const float time = c.a + (float)((tiles(c, M, N, E) + cus - 1) / cus) * (c.b + c.d * k);
-    if (f == 0 || time < least) {
+  for (int f = 0; f < kF8Forms; ++f) {
+    if ((kF8Have[ex][b16] >> f & 1) == 0) continue;
+    const F8Cost& c = kF8Cost[ex][b16][f];
+    float n = rows(kF8Shape[f].bm) * (float)((N + kF8Shape[f].bn - 1) / kF8Shape[f].bn) / cus;
+    if (!ex || n < 4.0f) n = std::ceil(n);         // whole rounds, where the number of tiles is known
+    const float time = c.a + n * (c.b + c.d * k);
+    if (best < 0 || time < least) {
       least = time;
       best = f;
     }
@@ -38,17 +55,15 @@ static int f8_best(int K, bool b16, int64_t (*tiles)(const F8Form&, int64_t, int
   return best;
 }
 static int choose_f8(int M, int N, int K, bool b16) {
-  return f8_best(K, b16, [](const F8Form& c, int64_t M, int64_t N, int64_t) {
-    return (M + c.bm - 1) / c.bm * ((N + c.bn - 1) / c.bn);
-  }, M, N, 1);
+  return f8_best(0, b16, N, K, [&](int bm) { return (float)((M + bm - 1) / bm); });
 }
-// As if each expert that can have a row had the mean of the rows.
+// As if the pairs fell on the experts evenly: so many are hit, and a hit one's rows end half-way through a tile.
 static int choose_f8_experts(int M, int N, int K, int E, bool b16) {
-  return f8_best(K, b16, [](const F8Form& c, int64_t M, int64_t N, int64_t E) {
-    const int64_t hit = std::min(M, E), rows = (M + hit - 1) / hit;
-    return hit * ((rows + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
-  }, M, N, E);
+  const float hit = E == 1 ? 1.0f : (float)E * (1.0f - std::exp(-(float)M / (float)E)), mean = (float)M / hit;
+  return f8_best(1, b16, N, K, [&](int bm) { return hit * (mean <= 0.7f * (float)bm ? 1.0f : mean / (float)bm + 0.5f); });
 }
+
+static int f8_streams(int64_t M, int64_t N, int out_dtype) { return M * N * (out_dtype == DT_F32 ? 4 : 2) > 32 << 20; }
 
 static int f8_fail(const char* what, const char* why) {
   set_error(std::string(what) + ": " + why);
@@ -66,7 +81,7 @@ static int f8_check(const char* what, const F8Args& a) {
   if (!al(a.x, 16) || !al(a.w, 16) || a.x_stride % 16 || a.w_stride % 16 || a.w_estride % 16 || a.x_stride < a.K || a.w_stride < a.K)
     return f8_fail(what, "code rows must start on 16 bytes, with strides of at least K");
   if (a.x_stride > kF8MaxStride || a.w_stride > kF8MaxStride) return f8_fail(what, "row strides go to 2^24 - 16");
-  if (a.sx_m < 0 || a.sx_b < 0) return f8_fail(what, "a scale stride is negative");
+  if (a.sx_m < 0 || a.sx_b < 0 || a.sx_m >= 1 << 22) return f8_fail(what, "scale strides are not negative, between rows below 2^22");
   if (!al(a.sx, 4) || !al(a.sw, 4) || !al(a.bias, 4) || !al(a.out, a.out_dtype == DT_F32 ? 4 : 2))
     return f8_fail(what, "scales, bias and output must be aligned to their element");
   if (a.out_stride < a.N && a.M > 1) return f8_fail(what, "output rows overlap");
@@ -87,12 +102,12 @@ int fp4x_f8_linear(const void* xq, int64_t x_stride, const float* xs, int64_t xs
                    int64_t w_stride, const float* ws, const float* bias, void* out, int64_t out_stride, int out_dtype,
                    int M, int N, int K, void* stream) {
   F8Args a{static_cast<const uint8_t*>(xq), x_stride, xs, xs_row, xs_block, static_cast<const uint8_t*>(wq), w_stride,
-           ws, bias, out, out_dtype, out_stride, M, N, K, 0, 0, 0, nullptr, nullptr, 1, M, 0};
+           ws, bias, out, out_dtype, out_stride, M, N, K, 0, 0, 0, f8_streams(M, N, out_dtype), nullptr, nullptr, 1, M, 0};
   if (int rc = f8_check("f8_linear", a)) return rc;
   if (M == 0) return FP4X_OK;
   const bool b16 = out_dtype == DT_F32;
   const int form = choose_f8(M, N, K, b16);
-  const F8Form& f = kF8Forms[form];
+  const F8Form& f = kF8Shape[form];
   a.mt = (M + f.bm - 1) / f.bm;
   a.nt = (N + f.bn - 1) / f.bn;
   a.gm = f.ring ? a.mt : 4;                        // 4 x 8 tiles of 256 x 256 are what the CUs of an XCD work on
@@ -115,7 +130,7 @@ int fp4x_f8_linear_experts(const void* xq, int64_t x_stride, const float* xs, in
                            int N, int K, void* stream) {
   const char* what = "f8_linear_experts";
   F8Args a{static_cast<const uint8_t*>(xq), x_stride, xs, xs_row, xs_block, static_cast<const uint8_t*>(wq), w_stride,
-           ws, nullptr, out, out_dtype, out_stride, P, N, K, 0, 0, 0, offsets, tokens, E, X, w_expert};
+           ws, nullptr, out, out_dtype, out_stride, P, N, K, 0, 0, 0, f8_streams(P, N, out_dtype), offsets, tokens, E, X, w_expert};
   if (E < 1 || E > kF8MaxExperts) return f8_fail(what, "1 to 4096 experts");
   if (int rc = f8_check(what, a)) return rc;
   if (P == 0) return FP4X_OK;
@@ -124,18 +139,20 @@ int fp4x_f8_linear_experts(const void* xq, int64_t x_stride, const float* xs, in
   if (w_expert < 0) return f8_fail(what, "a weight's stride is negative");
   if (tokens) {
     if (X < 1) return f8_fail(what, "there are no rows to pick from");
-    if ((int64_t)X * x_stride > (int64_t)UINT32_MAX) return f8_fail(what, "rows that are picked lie within 2^32 bytes");
+    if ((int64_t)X * x_stride > (int64_t)UINT32_MAX || (int64_t)X * xs_row * 4 > (int64_t)UINT32_MAX) return f8_fail(what, "rows that are picked, and their scales, lie within 2^32 bytes");
   } else if (X < P) {
     return f8_fail(what, "fewer rows than the output has");
   }
   const bool b16 = out_dtype == DT_F32;
   const int form = choose_f8_experts(P, N, K, E, b16);
-  const F8Form& f = kF8Forms[form];
+  const F8Form& f = kF8Shape[form];
   a.nt = (N + f.bn - 1) / f.bn;
   // every expert with a row may end in a tile of its own that is not full
   const int64_t hit = std::min(P, E), tiles = ((P - hit) / f.bm + hit) * a.nt;
-  if (tiles > INT32_MAX) return f8_fail(what, "more than 2^31 - 1 tiles");
-  (b16 ? launch_f8_experts_b16 : launch_f8_experts)(form, dim3((unsigned)tiles), a, (hipStream_t)stream);
+  if (tiles > INT32_MAX - 7) return f8_fail(what, "more than 2^31 - 8 tiles");
+  // large tiles: a workgroup takes several, 34 at most (lane j of its waves holds the place of tile j)
+  const int64_t slots = f.slots * device_cus(), grid = f.ring ? tiles : std::min(tiles, std::max(slots, (tiles + 31) / 32));
+  (b16 ? launch_f8_experts_b16 : launch_f8_experts)(form, dim3((unsigned)((grid + 7) / 8 * 8)), a, (hipStream_t)stream);
   return check_launch(what);
 }
 
