@@ -27,130 +27,186 @@ static int ex_fail(const char* what, const char* why) {
 }
 
 // ------------------------------------------------------------------ sort
-// A counting sort.  A workgroup takes a chunk of consecutive pairs, each of its
-// waves a part of that: counts per wave and expert in LDS, their sums over the
-// waves before, and then every wave walks its pairs again, 64 at a time, and
-// gives each the next place of its expert; within the 64 a pair's place is the
-// number of lanes before it with the same id.
+// A counting sort.  A workgroup takes a chunk of consecutive pairs, each of its W
+// counting waves a run of that, 256 at a time, four ids per lane: counts per wave
+// and expert in LDS, their sums over the waves before (a thread per expert), and
+// then every wave gives its pairs, 64 at a time, the next places of their experts;
+// within the 64 a pair's place is the number of lanes before it with the same id.
 //
-// Up to kSortOne pairs one workgroup does all.  Above, a first launch counts
-// per chunk, and in the second each workgroup adds up the chunks before its own
-// and the totals (at most 256 chunks of E counts, from L2).
-constexpr int kSortOne = 4096, kSortChunks = 256, kSortLds = 128 * 1024;
+// Up to 256 W pairs one workgroup does all, and its ids stay in registers between
+// the two passes.  Above, a first launch counts per chunk, and in the second each
+// workgroup adds up the chunks before its own and the totals (at most kSortChunks
+// of E counts, from L2).
+constexpr int kSortOne = 4096, kSortChunks = 256;
 
 struct SortArgs {
   const void* ids;  int wide;  int64_t row;        // int64 or int32, elements between tokens
-  int P, k, E, W, chunk, chunks;                   // W: waves per workgroup
+  int P, k, E, rounds, chunks;                     // rounds of 256 pairs per wave and chunk
   int* hist;                                       // [chunks][E]
   int *offsets, *tokens, *slots;
 };
 
-__device__ __forceinline__ int sort_id(const SortArgs& a, int p) {   // E: none
-  const int t = (int)((unsigned)p / (unsigned)a.k);
-  const int64_t at = t * a.row + (p - t * a.k);
-  const int64_t id = a.wide ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
-  return id >= 0 && id < a.E ? (int)id : a.E;
+struct SortRun {                                   // a wave's pairs [p0, p1)
+  int p0, p1;
+  __device__ SortRun(const SortArgs& a, int W) {
+    const int wave = threadIdx.x >> 6;
+    const int64_t lo = ((int64_t)blockIdx.x * W + wave) * 256 * a.rounds;
+    p0 = wave < W ? (int)min(lo, (int64_t)a.P) : a.P;
+    p1 = wave < W ? (int)min(lo + 256 * a.rounds, (int64_t)a.P) : a.P;
+  }
+};
+// Ids of pairs p, p + 64, .. (E: none, or past p1).
+__device__ __forceinline__ void sort_ids(const SortArgs& a, int p, int p1, int (&id)[4]) {
+  int64_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int q = p + 64 * i;
+    v[i] = -1;
+    if (q < p1) {
+      int64_t at = q;
+      if (a.row != a.k) at = (unsigned)q / (unsigned)a.k * a.row + (unsigned)q % (unsigned)a.k;
+      v[i] = a.wide ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) id[i] = v[i] >= 0 && v[i] < a.E ? (int)v[i] : a.E;
 }
-// Counts of this chunk's pairs per wave and expert.
-__device__ __forceinline__ void sort_count(const SortArgs& a, int p0, int p1, int* cnt) {
-  for (int i = threadIdx.x; i < a.W * a.E; i += 64 * a.W) cnt[i] = 0;
-  __syncthreads();
+template <int W>
+__device__ __forceinline__ void sort_count(const SortArgs& a, const SortRun& run, int* cnt, int (&id)[4]) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int p = p0 + lane; p < p1; p += 64) {
-    const int id = sort_id(a, p);
-    if (id < a.E) atomicAdd(&cnt[wave * a.E + id], 1);
+  sort_ids(a, run.p0 + lane, run.p1, id);          // on their way while the counts are cleared
+  for (int i = threadIdx.x; i < W * a.E; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  for (int r = 0; run.p0 + r * 256 < run.p1; ++r) {
+    if (r) sort_ids(a, run.p0 + r * 256 + lane, run.p1, id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (id[i] < a.E) atomicAdd(&cnt[wave * a.E + id[i]], 1);
   }
   __syncthreads();
 }
-__device__ __forceinline__ void sort_part(const SortArgs& a, int chunk, int& p0, int& p1) {
-  const int per = ((a.chunk + a.W - 1) / a.W + 63) & -64, wave = threadIdx.x >> 6;
-  const int64_t c0 = (int64_t)chunk * a.chunk, end = min(c0 + a.chunk, (int64_t)a.P), lo = c0 + (int64_t)wave * per;
-  p0 = (int)min(lo, end);
-  p1 = (int)min(lo + per, end);
-}
 
+template <int W>
 __global__ __launch_bounds__(1024) void sort_count_kernel(const SortArgs a) {
   extern __shared__ int cnt[];
-  int p0, p1;
-  sort_part(a, blockIdx.x, p0, p1);
-  sort_count(a, p0, p1, cnt);
-  for (int e = threadIdx.x; e < a.E; e += 64 * a.W) {
+  const SortRun run(a, W);
+  int id[4];
+  sort_count<W>(a, run, cnt, id);
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
     int n = 0;
-    for (int w = 0; w < a.W; ++w) n += cnt[w * a.E + e];
+#pragma unroll
+    for (int w = 0; w < W; ++w) n += cnt[w * a.E + e];
     a.hist[(int64_t)blockIdx.x * a.E + e] = n;
   }
 }
 
+template <int W>
 __global__ __launch_bounds__(1024) void sort_place_kernel(const SortArgs a) {
   extern __shared__ int cnt[];
   __shared__ int wave_total[16];
-  int p0, p1;
-  sort_part(a, blockIdx.x, p0, p1);
-  sort_count(a, p0, p1, cnt);
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, threads = 64 * a.W;
+  const SortRun run(a, W);
+  int id[4];
+  sort_count<W>(a, run, cnt, id);
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, waves = blockDim.x >> 6;
   int carry = 0;
-  for (int e0 = 0; e0 < a.E; e0 += threads) {      // a thread per expert
+  for (int e0 = 0; e0 < a.E; e0 += blockDim.x) {
     const int e = e0 + t;
-    int before = 0, total = 0, own = 0;
+    int before = 0, total = 0, n[W] = {};
     if (e < a.E) {
-      for (int w = 0; w < a.W; ++w) {
-        const int n = cnt[w * a.E + e];
-        cnt[w * a.E + e] = own;
-        own += n;
-      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) n[w] = cnt[w * a.E + e];
       if (a.chunks == 1) {
-        total = own;
+#pragma unroll
+        for (int w = 0; w < W; ++w) total += n[w];
       } else {
 #pragma unroll 8
         for (int c = 0; c < a.chunks; ++c) {
-          const int n = a.hist[(int64_t)c * a.E + e];
-          total += n;
-          if (c < (int)blockIdx.x) before += n;
+          const int m = a.hist[(int64_t)c * a.E + e];
+          total += m;
+          if (c < (int)blockIdx.x) before += m;
         }
       }
     }
     const int upto = wave_sum_to(total);
     if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
-    int base = carry;
-    for (int w = 0; w < a.W; ++w) {
-      const int n = wave_total[w];
-      if (w < wave) base += n;
-      carry += n;
-    }
-    base += upto - total;                          // where expert e begins
+    const int of = lane < waves ? wave_total[lane] : 0, to = wave_sum_to(of);   // the waves' totals, on every wave's lanes
+    const int base = carry + __builtin_amdgcn_readlane(to - of, __builtin_amdgcn_readfirstlane(wave)) + upto - total;
+    carry += __builtin_amdgcn_readlane(to, 63);
     if (e < a.E) {
-      if (blockIdx.x == 0) a.offsets[e] = base;
-      for (int w = 0; w < a.W; ++w) cnt[w * a.E + e] += base + before;
+      if (blockIdx.x == 0) a.offsets[e] = base;    // where expert e begins
+      int at = base + before;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        cnt[w * a.E + e] = at;
+        at += n[w];
+      }
     }
     __syncthreads();
   }
   if (blockIdx.x == 0 && t == 0) a.offsets[a.E] = carry;
   volatile int* next = cnt + wave * a.E;           // (a wave's LDS operations are done in order)
-  for (int p = p0 + lane; p - lane < p1; p += 64) {
-    const int id = p < p1 ? sort_id(a, p) : a.E;
-    const bool has = id < a.E;
-    uint64_t same = __ballot(has);
-    for (int b = 0; b < 32 - __builtin_clz(a.E); ++b) {
-      const uint64_t m = __ballot(has && (id >> b & 1));
-      same &= id >> b & 1 ? m : ~m;
-    }
-    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
-    if (has) {
-      const int at = next[id];
-      if (rank == 0) next[id] = at + __popcll(same);
-      a.tokens[at + rank] = (int)((unsigned)p / (unsigned)a.k);
-      a.slots[p] = at + rank;
-    } else if (p < p1) {
-      a.slots[p] = -1;
+  const int bits = 32 - __builtin_clz(a.E);
+  for (int r = 0; run.p0 + r * 256 < run.p1; ++r) {
+    if (a.rounds > 1) sort_ids(a, run.p0 + r * 256 + lane, run.p1, id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = run.p0 + r * 256 + 64 * i + lane;
+      if (p - lane >= run.p1) break;
+      const bool has = id[i] < a.E;
+      uint64_t same = __ballot(has);
+      for (int b = 0; b < bits; ++b) {
+        const uint64_t m = __ballot(has && (id[i] >> b & 1));
+        same &= id[i] >> b & 1 ? m : ~m;
+      }
+      const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+      if (has) {
+        const int at = next[id[i]];
+        if (rank == 0) next[id[i]] = at + __popcll(same);
+        a.tokens[at + rank] = (int)((unsigned)p / (unsigned)a.k);
+        a.slots[p] = at + rank;
+      } else if (p < run.p1) {
+        a.slots[p] = -1;
+      }
     }
   }
-  for (int64_t s = carry + (int64_t)blockIdx.x * threads + t; s < a.P; s += (int64_t)gridDim.x * threads) a.tokens[s] = -1;
+  for (int64_t s = carry + (int64_t)blockIdx.x * blockDim.x + t; s < a.P; s += (int64_t)gridDim.x * blockDim.x) a.tokens[s] = -1;
+}
+
+// Chunks of W waves; W by the pairs (few pairs: few counts to clear and to add) and by the LDS that E counts per wave take.
+struct SortPlan {
+  int W, rounds, chunks;
+  SortPlan(int64_t P, int E) : W(P <= 256 ? 1 : P <= 1024 ? 4 : E <= 2048 ? 16 : 8), rounds(1), chunks(1) {
+    if (P > kSortOne || P > 256 * W) {
+      rounds = (int)((P + (int64_t)kSortChunks * 256 * W - 1) / ((int64_t)kSortChunks * 256 * W));
+      chunks = (int)((P + (int64_t)256 * W * rounds - 1) / ((int64_t)256 * W * rounds));
+    }
+  }
+};
+template <int W>
+static int launch_sort(const SortArgs& a, hipStream_t st) {
+  const int lds = W * a.E * (int)sizeof(int);
+  const dim3 grid(a.chunks), threads(std::max(64 * W, std::min(1024, (a.E + 63) / 64 * 64)));
+  if (lds > 48 * 1024)
+    for (const void* f : {reinterpret_cast<const void*>(sort_count_kernel<W>), reinterpret_cast<const void*>(sort_place_kernel<W>)})
+      if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return check_launch("expert_sort");
+  if (a.chunks > 1) hipLaunchKernelGGL((sort_count_kernel<W>), grid, threads, lds, st, a);
+  hipLaunchKernelGGL((sort_place_kernel<W>), grid, threads, lds, st, a);
+  return check_launch("expert_sort");
 }
 
 // ------------------------------------------------------------------ rows
 // Bytes are copied as they are, 16 at a time, the last 16 of a row again where
 // its length is no multiple.  A wave takes up to kRowPart bytes of a row.
+//
+// Experts share tokens: each row of x is read k times, by rows of the output that
+// lie far apart.  So where that is four times or more, and the output is larger
+// than the L2, an XCD (workgroups go
+// to the eight in turn) takes the rows whose tokens are in its eighth of x, which
+// its L2 keeps, and the output passes by: for each 16 rows, each XCD has a wave
+// that copies its own of them.  32768 rows of 2560 in bf16 took 48 us without this
+// (40 with it), 131072 of 1024 79 (58); at two rows per token it loses (26 against
+// 33 at 8192 of 5120).
 constexpr int kRowPart = 8192;
 typedef uint32_t u32x4_b __attribute__((ext_vector_type(4), aligned(1)));
 
@@ -161,30 +217,56 @@ struct RowsArgs {
   int T, P, parts;
   int64_t bytes;
 };
+template <bool STREAM>
+__device__ __forceinline__ void copy_row(const RowsArgs& a, int lane, int64_t s, int tok, int part) {
+  const int64_t b0 = (int64_t)part * kRowPart, n = min(a.bytes - b0, (int64_t)kRowPart);
+  const bool has = tok >= 0 && tok < a.T;
+  const uint8_t* from = a.x + (int64_t)(has ? tok : 0) * a.x_stride + b0;
+  uint8_t* to = a.out + s * a.out_stride + b0;
+  if (n < 16) {
+    if (lane < n) to[lane] = has ? from[lane] : 0;
+    return;
+  }
+  for (int64_t b = lane * 16; b - lane * 16 < n; b += 4096) {
+    u32x4_b v[4];
+    if (has) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const u32x4_b*>(from + min(b + i * 1024, n - 16));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = u32x4_b{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4_b* p = reinterpret_cast<u32x4_b*>(to + min(b + i * 1024, n - 16));
+      if (b + i * 1024 < n) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v[i], p);
+        else *p = v[i];
+      }
+    }
+  }
+}
 __global__ __launch_bounds__(256) void expert_rows_kernel(const RowsArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * 4, items = (int64_t)a.P * a.parts;
-  for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += waves) {
-    const int64_t s = it / a.parts, b0 = (it - s * a.parts) * kRowPart, n = min(a.bytes - b0, (int64_t)kRowPart);
-    const int tok = a.tokens[s];
-    const bool has = tok >= 0 && tok < a.T;
-    const uint8_t* from = a.x + (int64_t)(has ? tok : 0) * a.x_stride + b0;
-    uint8_t* to = a.out + s * a.out_stride + b0;
-    if (n < 16) {
-      if (lane < n) to[lane] = has ? from[lane] : 0;
-      continue;
-    }
-    u32x4_b v[kRowPart / 1024];
-#pragma unroll
-    for (int i = 0; i < kRowPart / 1024; ++i) {
-      const int64_t at = (i * 64 + lane) * 16;
-      v[i] = u32x4_b{0, 0, 0, 0};
-      if (has && i * 1024 < n) v[i] = *reinterpret_cast<const u32x4_b*>(from + min(at, n - 16));
-    }
-#pragma unroll
-    for (int i = 0; i < kRowPart / 1024; ++i) {
-      const int64_t at = (i * 64 + lane) * 16;
-      if (at < n) *reinterpret_cast<u32x4_b*>(to + min(at, n - 16)) = v[i];
+  for (int64_t it = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); it < items; it += waves) {
+    const int64_t s = it / a.parts;
+    copy_row<false>(a, lane, s, a.tokens[s], (int)(it - s * a.parts));
+  }
+}
+__global__ __launch_bounds__(256) void expert_rows_large_kernel(const RowsArgs a) {
+  const int lane = threadIdx.x & 63, xcd = blockIdx.x & 7;
+  const int lo = (int)((int64_t)a.T * xcd >> 3), hi = (int)((int64_t)a.T * (xcd + 1) >> 3);
+  const int64_t waves = (int64_t)(gridDim.x >> 3) * 4, items = (((int64_t)a.P + 15) >> 4) * a.parts;   // (the grid is a multiple of 8)
+  for (int64_t it = (int64_t)(blockIdx.x >> 3) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); it < items; it += waves) {
+    const int64_t g = it / a.parts, s = g * 16 + lane;
+    const int tok = lane < 16 && s < a.P ? a.tokens[s] : -1;
+    const bool none = tok < 0 || tok >= a.T;       // zeros: dealt by their place
+    uint64_t mine = __ballot(lane < 16 && s < a.P && (none ? (lane & 7) == xcd : tok >= lo && tok < hi));
+    while (mine) {
+      const int l = __builtin_ctzll(mine);
+      mine &= mine - 1;
+      copy_row<true>(a, lane, g * 16 + l, __builtin_amdgcn_readlane(tok, l), (int)(it - g * a.parts));
     }
   }
 }
@@ -243,9 +325,10 @@ struct CombineArgs {
   int T, k, P, H, parts;                           // parts: waves per token
 };
 
-// A wave takes 512 values of a token, eight per lane, and its k rows eight at a time, whose loads are on their way
-// together.  The last lanes of a row are moved back to end at H.
-template <int DT>
+// A wave takes 512 values of a token, eight per lane, and its k rows B at a time, whose loads are on their way together (B 8
+// for two rows left registers for 5 waves per SIMD: 20000 tokens of 2 rows of 700 took 34 us).  The last lanes of a row are
+// moved back to end at H.
+template <int DT, int B>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const CombineArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * 4, items = (int64_t)a.T * a.parts;
@@ -267,25 +350,33 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const CombineArgs a
     }
     const int h = min(h0, a.H - 8);
     float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j0 = 0; j0 < a.k; j0 += 8) {
-      Vec8<DT> v[8];
-      float w[8];
-      bool has[8];
+    for (int j0 = 0; j0 < a.k; j0 += B) {
+      Vec8<DT> v[B];
+      float w[B];
+      bool has[B];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < B; ++j) {
         const int at = min(j0 + j, a.k - 1), s = slots[at];
         has[j] = j0 + j < a.k && s >= 0 && s < a.P;
         if (has[j]) v[j].load(a.y, s * a.y_stride + h);
         w[j] = a.w ? weight_at(a.w, a.w_dtype, t * a.k + at) : 1.0f;
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < B; ++j)
         if (has[j])
 #pragma unroll
           for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w[j], v[j].get(i), acc[i]);
     }
     if (h0 < a.H) put8<DT>(a.out, t * a.out_stride + h, acc);
   }
+}
+
+template <int DT>
+static void launch_combine(const CombineArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.T * a.parts + 3) / 4, 1 << 20));
+  if (a.k <= 2) hipLaunchKernelGGL((expert_combine_kernel<DT, 2>), grid, dim3(256), 0, st, a);
+  else if (a.k <= 4) hipLaunchKernelGGL((expert_combine_kernel<DT, 4>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((expert_combine_kernel<DT, 8>), grid, dim3(256), 0, st, a);
 }
 
 // ------------------------------------------------------------------ its gradient
@@ -303,8 +394,23 @@ struct GradArgs {
 
 // A workgroup takes a token: its row of dout stays in registers, C chunks of
 // eight values per lane, while its k rows of y go by.  A wave's sum of the
-// products is a butterfly, the waves' are added in their order.  Workgroups past
+// products has a fixed order, and the waves' are added in theirs.  Workgroups past
 // the tokens clear the rows that no pair has.
+// A sum over the wave, in a fixed order: within 16 lanes, then of the four 16s, in lane 63's place.
+__device__ __forceinline__ float wave_total(float v) {
+  const auto other = [](float x, auto ctrl, auto rows) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  v += other(v, integral_constant<int, 0x111>(), integral_constant<int, 0xf>());
+  v += other(v, integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  v += other(v, integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  v += other(v, integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  v += other(v, integral_constant<int, 0x142>(), integral_constant<int, 0xa>());
+  v += other(v, integral_constant<int, 0x143>(), integral_constant<int, 0xc>());
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 template <int DT, int C>
 __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
   __shared__ float sum[16][kGradTop];
@@ -345,28 +451,42 @@ __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
     h[c] = min(h0, a.H - 8);
     d[c].load(a.d, tok * a.d_stride + h[c]);
   }
-  for (int j = 0; j < a.k; ++j) {
-    const int s = slots[j];
-    float dot = 0.0f;
-    if (s >= 0 && s < a.P) {
-      const float w = weight_at(a.w, a.w_dtype, tok * a.k + j);
-      Vec8<DT> v[C];
+  constexpr int B = C == 1 ? 4 : C == 2 ? 2 : 1;   // rows whose loads are on their way together
+  for (int j0 = 0; j0 < a.k; j0 += B) {
+    Vec8<DT> v[B][C];
+    int s[B];
+    float dot[B], w[B];
 #pragma unroll
-      for (int c = 0; c < C; ++c) v[c].load(a.y, s * a.y_stride + h[c]);
+    for (int j = 0; j < B; ++j) {
+      const int at = min(j0 + j, a.k - 1);
+      s[j] = slots[at];
+      if (j0 + j >= a.k || s[j] >= a.P) s[j] = -1;
+      w[j] = weight_at(a.w, a.w_dtype, tok * a.k + at);
+      if (s[j] >= 0)
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int dup = (c * (int)blockDim.x + t) * 8 - h[c];   // values that the chunk before has, of one moved back
-        float g[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          g[i] = w * d[c].get(i);
-          if (in[c] && i >= dup) dot = __builtin_fmaf(d[c].get(i), v[c].get(i), dot);
-        }
-        if (in[c]) put8<DT>(a.dy, s * a.dy_stride + h[c], g);
-      }
+        for (int c = 0; c < C; ++c) v[j][c].load(a.y, s[j] * a.y_stride + h[c]);
     }
-    dot = group_allreduce(dot, 64);
-    if (lane == 0) sum[wave][j] = dot;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      dot[j] = 0.0f;
+      if (s[j] >= 0)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int dup = (c * (int)blockDim.x + t) * 8 - h[c];   // values that the chunk before has, of one moved back
+          float g[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            g[i] = w[j] * d[c].get(i);
+            if (in[c] && i >= dup) dot[j] = __builtin_fmaf(d[c].get(i), v[j][c].get(i), dot[j]);
+          }
+          if (in[c]) put8<DT>(a.dy, s[j] * a.dy_stride + h[c], g);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const float total = wave_total(dot[j]);
+      if (lane == 0 && j0 + j < a.k) sum[wave][j0 + j] = total;
+    }
   }
   __syncthreads();
   for (int j = t; j < a.k; j += blockDim.x) {
@@ -397,10 +517,9 @@ using namespace fp4x;
 extern "C" {
 
 int64_t fp4x_expert_sort_workspace(int64_t T, int k, int E) {
-  const int64_t P = T * k;
-  if (P <= kSortOne) return 0;
-  const int64_t chunk = std::max<int64_t>(kSortOne, ((P + kSortChunks - 1) / kSortChunks + 1023) / 1024 * 1024);
-  return (P + chunk - 1) / chunk * E * (int64_t)sizeof(int);
+  if (T < 1 || k < 1 || E < 1) return 0;
+  const SortPlan plan(T * k, E);
+  return plan.chunks == 1 ? 0 : (int64_t)plan.chunks * E * (int64_t)sizeof(int);
 }
 
 int fp4x_expert_sort(const void* ids, int wide, int64_t row, int64_t T, int k, int E, int* offsets, int* tokens,
@@ -416,24 +535,13 @@ int fp4x_expert_sort(const void* ids, int wide, int64_t row, int64_t T, int k, i
   const int64_t need = fp4x_expert_sort_workspace(T, k, E);
   if (need && (!workspace || workspace_bytes < need || !al4(workspace))) return ex_fail(what, "the workspace is too small, null or misaligned");
   const int P = (int)(T * k);
-  int W = std::min(16, std::max(1, kSortLds / 4 / E));
-  if (P <= 2048) W = std::min(W, std::max(1, (P + 255) / 256 * 2));       // few pairs: few counts to clear and to add
-  SortArgs a{ids, wide ? 1 : 0, row, P, k, E, W, 0, 1, static_cast<int*>(workspace), offsets, tokens, slots};
+  const SortPlan plan(P, E);
+  const SortArgs a{ids, wide ? 1 : 0, row, P, k, E, plan.rounds, plan.chunks, static_cast<int*>(workspace), offsets, tokens, slots};
   hipStream_t st = (hipStream_t)stream;
-  if (need) {
-    a.chunk = std::max(kSortOne, ((P + kSortChunks - 1) / kSortChunks + 1023) / 1024 * 1024);
-    a.chunks = (P + a.chunk - 1) / a.chunk;
-  } else {
-    a.chunk = (std::max(P, 1) + 64 * W - 1) / (64 * W) * (64 * W);
-  }
-  const int lds = W * E * (int)sizeof(int);
-  if (lds > 48 * 1024) {
-    for (const void* f : {reinterpret_cast<const void*>(sort_count_kernel), reinterpret_cast<const void*>(sort_place_kernel)})
-      if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return check_launch(what);
-  }
-  if (need) hipLaunchKernelGGL(sort_count_kernel, dim3(a.chunks), dim3(64 * W), lds, st, a);
-  hipLaunchKernelGGL(sort_place_kernel, dim3(a.chunks), dim3(64 * W), lds, st, a);
-  return check_launch(what);
+  if (plan.W == 1) return launch_sort<1>(a, st);
+  if (plan.W == 4) return launch_sort<4>(a, st);
+  if (plan.W == 8) return launch_sort<8>(a, st);
+  return launch_sort<16>(a, st);
 }
 
 int fp4x_expert_rows(const void* x, int64_t x_stride, int elem, int T, const int* tokens, int P, int H, void* out,
@@ -447,8 +555,13 @@ int fp4x_expert_rows(const void* x, int64_t x_stride, int elem, int T, const int
   const int64_t parts = (bytes + kRowPart - 1) / kRowPart;
   const RowsArgs a{static_cast<const uint8_t*>(x), x_stride * elem, tokens, static_cast<uint8_t*>(out), out_stride * elem,
                    T, P, (int)parts, bytes};
-  const dim3 grid((unsigned)std::min<int64_t>((P * parts + 3) / 4, 1 << 20));
-  hipLaunchKernelGGL(expert_rows_kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
+  hipStream_t st = (hipStream_t)stream;
+  if (P / 4 >= T && T >= 8 && P * bytes > 32 << 20) {
+    const dim3 grid((unsigned)std::min<int64_t>((((int64_t)P + 15) / 16 * parts + 3) / 4, 1 << 17) * 8);
+    hipLaunchKernelGGL(expert_rows_large_kernel, grid, dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(expert_rows_kernel, dim3((unsigned)std::min<int64_t>((P * parts + 3) / 4, 1 << 20)), dim3(256), 0, st, a);
+  }
   return check_launch(what);
 }
 
@@ -463,11 +576,10 @@ int fp4x_expert_combine(const void* y, int64_t y_stride, int dtype, int P, const
   if (y_stride < 0 || (T > 1 && out_stride < H)) return ex_fail(what, "output rows overlap, or a stride is negative");
   const int parts = (H + 511) / 512;
   const CombineArgs a{y, y_stride, slots, w, w_dtype, out, out_stride, T, k, P, H, parts};
-  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)T * parts + 3) / 4, 1 << 20));
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_BF16) hipLaunchKernelGGL((expert_combine_kernel<DT_BF16>), grid, dim3(256), 0, st, a);
-  else if (dtype == DT_F16) hipLaunchKernelGGL((expert_combine_kernel<DT_F16>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((expert_combine_kernel<DT_F32>), grid, dim3(256), 0, st, a);
+  if (dtype == DT_BF16) launch_combine<DT_BF16>(a, st);
+  else if (dtype == DT_F16) launch_combine<DT_F16>(a, st);
+  else launch_combine<DT_F32>(a, st);
   return check_launch(what);
 }
 
