@@ -312,12 +312,13 @@ int fp4x_quantize_f8(const void* w, int64_t w_row, int64_t w_expert, int dtype, 
  * ws[n / 128, b]) + bias[n]), b the blocks of 128 values of K: e4m3 codes, a
  * block's sum from the matrix cores, scaled and added in fp32.  For bf16 and fp16
  * outputs the products are the fp8 instruction's, which adds eight at a time, cut
- * to 2^-13 of the power of two of the largest; for fp32 outputs they are exact.  xs fp32 at
- * xs[m * xs_row + b * xs_block] (FP4X_Q8_E4M3_G128: xs_row 1, xs_block M; reads
- * of neighbouring rows are then one line), ws fp32 [ceil(N / 128), ceil(K /
- * 128)], bias fp32 [N] or NULL.  Code rows start on 16 bytes (strides a multiple
- * of 16, below 2^24) and are readable to the next 16-byte boundary past K; what
- * is there is ignored.  M and N go to 2^24, M N to 2^37, K to 2^24.  No
+ * to 2^-13 of the power of two of the largest; for fp32 outputs they are exact.
+ * xs fp32 at xs[m * xs_row + b * xs_block] (FP4X_Q8_E4M3_G128: xs_row 1, xs_block
+ * M; reads of neighbouring rows are then one line), ws fp32 [ceil(N / 128),
+ * ceil(K / 128)], bias fp32 [N] or NULL.  Code rows start on 16 bytes (strides a
+ * multiple of 16, below 2^24) and are readable to the next 16-byte boundary past
+ * K; what is there is ignored.  M and N go to 2^24, M N to 2^37, K to 131071, the
+ * tiles of the form to 2^24 - 9 (refused above); xs_row is below 2^22.  No
  * counterpart in the reference. */
 int fp4x_f8_linear(const void* xq, int64_t x_stride, const float* xs, int64_t xs_row, int64_t xs_block, const void* wq,
                    int64_t w_stride, const float* ws, const float* bias, void* out, int64_t out_stride, int out_dtype,
@@ -327,7 +328,8 @@ int fp4x_f8_linear(const void* xq, int64_t x_stride, const float* xs, int64_t xs
  * of xq [X, K] for output row s, or, where tokens is NULL, row s.  offsets int32
  * [E + 1] on the device, rising; they are cut to 0 .. P, and a token outside 0 ..
  * X - 1 to its ends.  Rows before offsets[0] and from offsets[E] on are not
- * written.  1 to 4096 experts; picked rows lie within 2^32 bytes. */
+ * written.  1 to 4096 experts; picked rows, and their scales, lie within 2^32
+ * bytes. */
 int fp4x_f8_linear_experts(const void* xq, int64_t x_stride, const float* xs, int64_t xs_row, int64_t xs_block, int X,
                            const int* tokens, const int* offsets, int E, const void* wq, int64_t w_stride,
                            int64_t w_expert, const float* ws, void* out, int64_t out_stride, int out_dtype, int P,
@@ -361,7 +363,8 @@ int fp4x_expert_combine(const void* y, int64_t y_stride, int dtype, int P, const
 /* Its gradients: dy[slots[t, j]] = w[t, j] dout[t], zeros in the rows s whose
  * tokens[s] is no token; dw[t, j] = dout[t] . y[slots[t, j]] (0 without a row).
  * No two slots are one row.  dy has y's dtype and shares no memory with anything
- * else, dw has w's.  k <= 128, H <= 32768. */
+ * else, dw has w's.  k <= 128, H <= 32768; tokens times the lanes of a row (H / 8
+ * in whole 64s, up to 1024) stay below 2^32. */
 int fp4x_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int dtype, int P,
                              const int* slots, const int* tokens, const void* w, int w_dtype, void* dy,
                              int64_t dy_stride, void* dw, int T, int k, int H, void* stream);

@@ -187,7 +187,7 @@ template <int W>
 static int launch_sort(const SortArgs& a, hipStream_t st) {
   const int lds = W * a.E * (int)sizeof(int);
   const dim3 grid(a.chunks), threads(std::max(64 * W, std::min(1024, (a.E + 63) / 64 * 64)));
-  if (lds > 48 * 1024)
+  if (lds >= 64 * 1024)                            // with the 64 bytes of wave_total
     for (const void* f : {reinterpret_cast<const void*>(sort_count_kernel<W>), reinterpret_cast<const void*>(sort_place_kernel<W>)})
       if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return check_launch("expert_sort");
   if (a.chunks > 1) hipLaunchKernelGGL((sort_count_kernel<W>), grid, threads, lds, st, a);
@@ -497,13 +497,16 @@ __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
 }
 
 template <int DT>
-static void launch_grad(const GradArgs& a, hipStream_t st) {
+static int launch_grad(const GradArgs& a, hipStream_t st) {
   const int chunks = (a.H + 7) / 8, C = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 4;
   const int threads = std::min(1024, ((chunks + C - 1) / C + 63) / 64 * 64);
-  const dim3 grid((unsigned)(a.T + (a.P + (int64_t)kGradTail - 1) / kGradTail));
+  const int64_t groups = a.T + (a.P + (int64_t)kGradTail - 1) / kGradTail;
+  if (groups * threads > (int64_t)UINT32_MAX) return ex_fail("expert_combine_grad", "tokens times the lanes of a row pass 2^32");
+  const dim3 grid((unsigned)groups);
   if (C == 1) hipLaunchKernelGGL((expert_grad_kernel<DT, 1>), grid, dim3(threads), 0, st, a);
   else if (C == 2) hipLaunchKernelGGL((expert_grad_kernel<DT, 2>), grid, dim3(threads), 0, st, a);
   else hipLaunchKernelGGL((expert_grad_kernel<DT, 4>), grid, dim3(threads), 0, st, a);
+  return check_launch("expert_combine_grad");
 }
 
 static bool ex_dt(int dt) { return dt == DT_BF16 || dt == DT_F32 || dt == DT_F16; }
@@ -596,13 +599,11 @@ int fp4x_expert_combine_grad(const void* dout, int64_t dout_stride, const void* 
       !ex_al(dw, w_dtype))
     return ex_fail(what, "tensors must be aligned to their element");
   if (dout_stride < 0 || y_stride < 0 || (P > 1 && dy_stride < H)) return ex_fail(what, "output rows overlap, or a stride is negative");
-  if (T + ((int64_t)P + kGradTail - 1) / kGradTail > INT32_MAX) return ex_fail(what, "too many rows");
   const GradArgs a{dout, dout_stride, y, y_stride, slots, tokens, w, w_dtype, dy, dy_stride, dw, T, k, P, H};
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_BF16) launch_grad<DT_BF16>(a, st);
-  else if (dtype == DT_F16) launch_grad<DT_F16>(a, st);
-  else launch_grad<DT_F32>(a, st);
-  return check_launch(what);
+  if (dtype == DT_BF16) return launch_grad<DT_BF16>(a, st);
+  if (dtype == DT_F16) return launch_grad<DT_F16>(a, st);
+  return launch_grad<DT_F32>(a, st);
 }
 
 }  // extern "C"

@@ -12,6 +12,8 @@ int device_cus();
 
 // ------------------------------------------------------------------ choice
 constexpr int64_t kF8MaxStride = (1 << 24) - 16;   // 256 rows within 32-bit offsets
+// A grid has fewer than 2^32 lanes, 256 a tile (forms of 512 have fewer tiles at every size that M N allows).
+constexpr int64_t kF8MaxTiles = (1 << 24) - 8;
 
 struct F8Form { int bm, bn, slots, ring, stages; };
 constexpr F8Form kF8Shape[kF8Forms] = {{16, 16, 2, 1, 2},   {16, 32, 2, 1, 3},   {32, 32, 2, 1, 2},   {32, 64, 1, 1, 2},
@@ -72,7 +74,7 @@ static int f8_fail(const char* what, const char* why) {
 
 // What both entry points ask of their arguments; 0 rows: nothing else is looked at.
 static int f8_check(const char* what, const F8Args& a) {
-  if (a.M < 0 || a.N < 1 || a.K < 1 || a.K > 1 << 24) return f8_fail(what, "need M >= 0, N >= 1 and 1 <= K <= 2^24");
+  if (a.M < 0 || a.N < 1 || a.K < 1 || a.K > 131071) return f8_fail(what, "need M >= 0, N >= 1 and 1 <= K <= 131071");
   if (a.out_dtype != DT_BF16 && a.out_dtype != DT_F32 && a.out_dtype != DT_F16) return f8_fail(what, "out is bf16, fp32 or fp16");
   if (a.M > 1 << 24 || a.N > 1 << 24 || (int64_t)a.M * a.N > (int64_t)1 << 37) return f8_fail(what, "M and N go to 2^24, M N to 2^37");
   if (a.M == 0) return FP4X_OK;
@@ -112,6 +114,7 @@ int fp4x_f8_linear(const void* xq, int64_t x_stride, const float* xs, int64_t xs
   a.nt = (N + f.bn - 1) / f.bn;
   a.gm = f.ring ? a.mt : 4;                        // 4 x 8 tiles of 256 x 256 are what the CUs of an XCD work on
   const int tiles = a.mt * a.nt, slots = f.slots * device_cus();
+  if (tiles >= kF8MaxTiles) return f8_fail("f8_linear", "2^24 tiles or more");
   // Several tiles per workgroup only where a tile has more k-tiles than the ring has stages: the bias of tile t + 2
   // takes the place of tile t's when the last load of tile t + 1 is out, which is then behind a barrier that every wave
   // comes to after its part of tile t's epilogue.
@@ -149,9 +152,9 @@ int fp4x_f8_linear_experts(const void* xq, int64_t x_stride, const float* xs, in
   a.nt = (N + f.bn - 1) / f.bn;
   // every expert with a row may end in a tile of its own that is not full
   const int64_t hit = std::min(P, E), tiles = ((P - hit) / f.bm + hit) * a.nt;
-  if (tiles > INT32_MAX - 7) return f8_fail(what, "more than 2^31 - 8 tiles");
   // large tiles: a workgroup takes several, 34 at most (lane j of its waves holds the place of tile j)
   const int64_t slots = f.slots * device_cus(), grid = f.ring ? tiles : std::min(tiles, std::max(slots, (tiles + 31) / 32));
+  if (grid >= kF8MaxTiles) return f8_fail(what, "2^24 tiles or more");
   (b16 ? launch_f8_experts_b16 : launch_f8_experts)(form, dim3((unsigned)((grid + 7) / 8 * 8)), a, (hipStream_t)stream);
   return check_launch(what);
 }
