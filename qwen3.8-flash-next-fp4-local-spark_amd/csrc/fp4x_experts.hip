@@ -37,6 +37,10 @@ static int ex_fail(const char* what, const char* why) {
 // the two passes.  Above, a first launch counts per chunk, and in the second each
 // workgroup adds up the chunks before its own and the totals (at most kSortChunks
 // of E counts, from L2).
+//
+// Bound by latency, not by its 24 bytes per pair: 24 pairs of 512 experts take 2.8
+// us, 32008 of 256 experts 4.8 + 7.5 in two launches, where the bytes are 0.2: a
+// kernel's start and reads that wait for each other (ids, the chunks' counts).
 constexpr int kSortOne = 4096, kSortChunks = 256;
 
 struct SortArgs {
@@ -201,11 +205,11 @@ static int launch_sort(const SortArgs& a, hipStream_t st) {
 //
 // Experts share tokens: each row of x is read k times, by rows of the output that
 // lie far apart.  So where that is four times or more, and the output is larger
-// than the L2, an XCD (workgroups go
-// to the eight in turn) takes the rows whose tokens are in its eighth of x, which
-// its L2 keeps, and the output passes by: for each 16 rows, each XCD has a wave
-// that copies its own of them.  32768 rows of 2560 in bf16 took 48 us without this
-// (40 with it), 131072 of 1024 79 (58); at two rows per token it loses (26 against
+// than the L2, an XCD (workgroups go to the eight in turn) takes the rows whose
+// tokens are in its eighth of x, which its L2 keeps, and the output passes by: for
+// each 16 rows, each XCD has a wave that copies its own of them.  32768 rows of
+// 2560 in bf16 took 48 us without this (40 with it: 188 MB at 4.7 TB/s, bound by
+// the writes), 131072 of 1024 79 (58); at two rows per token it loses (26 against
 // 33 at 8192 of 5120).
 constexpr int kRowPart = 8192;
 typedef uint32_t u32x4_b __attribute__((ext_vector_type(4), aligned(1)));
@@ -327,7 +331,8 @@ struct CombineArgs {
 
 // A wave takes 512 values of a token, eight per lane, and its k rows B at a time, whose loads are on their way together (B 8
 // for two rows left registers for 5 waves per SIMD: 20000 tokens of 2 rows of 700 took 34 us).  The last lanes of a row are
-// moved back to end at H.
+// moved back to end at H.  Sums are fp32 by fma, rounded once.  Bound by the reads: 4096 tokens of 8 rows of 2560 in bf16,
+// 189 MB, take 42 us (4.5 TB/s); 3 tokens 3.0 (latency).
 template <int DT, int B>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const CombineArgs a) {
   const int lane = threadIdx.x & 63;
@@ -392,10 +397,6 @@ struct GradArgs {
   int T, k, P, H;
 };
 
-// A workgroup takes a token: its row of dout stays in registers, C chunks of
-// eight values per lane, while its k rows of y go by.  A wave's sum of the
-// products has a fixed order, and the waves' are added in theirs.  Workgroups past
-// the tokens clear the rows that no pair has.
 // A sum over the wave, in a fixed order: within 16 lanes, then of the four 16s, in lane 63's place.
 __device__ __forceinline__ float wave_total(float v) {
   const auto other = [](float x, auto ctrl, auto rows) {
@@ -411,6 +412,12 @@ __device__ __forceinline__ float wave_total(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+// A workgroup takes a token: its row of dout stays in registers, C chunks of
+// eight values per lane, while its k rows of y go by, so that y is read and dy
+// written once for both gradients.  A wave's sum of the products has a fixed
+// order, and the waves' are added in theirs.  Workgroups past the tokens clear the
+// rows that no pair has.  Bound by memory: 4096 tokens of 8 rows of 2560 in bf16,
+// 357 MB, take 70 us (5.1 TB/s, a large copy's rate).
 template <int DT, int C>
 __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
   __shared__ float sum[16][kGradTop];

@@ -5,6 +5,12 @@
 // x 16 outputs, which starts at 0; it is scaled and added to the outputs' fp32
 // sums by fma in the order of the blocks.
 //
+// That instruction adds eight neighbouring products at a time, each cut to 2^-13
+// of the power of two of the largest (measured; v_mfma_f32_16x16x32_fp8_fp8 does
+// the same): 1.5e-5 of a block's sum of normal values, a thirtieth of fp16's half
+// step.  For fp32 outputs (B16) both operands are turned into bf16, which
+// holds every e4m3 value, and multiplied exactly, at half of the rate.
+//
 // The same over experts: rows [off[e], off[e + 1]) of the output are products
 // with expert e's weight, their rows of x picked by an index or lying in order.
 #pragma once
@@ -106,7 +112,7 @@ __device__ __forceinline__ int f8_expert_tiles(const F8Args& a, F8Place& p) {
   return tiles;
 }
 // The same for one tile per workgroup, which the lanes look up together: the second time each takes an expert (24 rows of
-// 512 experts took 18.1 us with the function above, 17.0 with this).
+// 512 experts on 16 x 32 tiles took 1.1 us more with the function above).
 template <int BM, int BN>
 __device__ __forceinline__ bool f8_expert_tile(const F8Args& a, F8Place& p) {
   const int lane = threadIdx.x & 63, per = (a.E + 63) >> 6;
@@ -194,7 +200,8 @@ __device__ __forceinline__ void f8_store4(const F8Args& a, int64_t m, int n, con
 }
 
 // 16 bytes of the output.  One that is larger than the 32 MB of the XCDs' L2 passes by it: it would push out the rows of x
-// and w that the next tiles share (4096 x [16384 x 2560] took 175 us so, 163 with these stores).
+// and w that the next tiles share (4096 x [16384 x 2560] took 175 us so, 163 with these stores).  Below that the next
+// launch finds its input in the caches.
 template <class V>
 __device__ __forceinline__ void f8_put(V* at, V v, int stream) {
   if (stream) asm volatile("global_store_dwordx4 %0, %1, off nt" ::"v"(at), "v"(v) : "memory");   // (two plain stores would be merged)
@@ -208,6 +215,11 @@ __device__ __forceinline__ void f8_put(V* at, V v, int stream) {
 // tiles do.  A unit's scales come with it (one more load: 16 MT of x, one of w,
 // whose 16 NT rows lie in one block).  The waves' fp32 sums meet in LDS in the
 // waves' order.
+//
+// Bound by the weight's bytes or by latency: 6 rows by [11316 x 9088], 103 MB, take
+// 19.3 us (5.3 TB/s; a large copy moves 5.1), 3 rows by [2560 x 640] 3.3.  K is
+// split over the W waves of a workgroup, D units of each on their way, and not over
+// workgroups, whose sums would take a second pass over memory.
 template <int MT, int NT, int W, int D, bool EX, bool B16>
 __global__ __launch_bounds__(64 * W, 2) void f8_ring_kernel(const F8Args a) {
   constexpr int R = 16 * (MT + NT), NL = R / 8, STAGE = R * 128 + 256;
@@ -349,6 +361,17 @@ __global__ __launch_bounds__(64 * W, 2) void f8_ring_kernel(const F8Args a) {
 // strip is read, and in the last one, behind the k-tile's only barrier, the
 // first of the next k-tile and its rows of w, each once its last MFMA is issued.
 // A block's sum is scaled and added two MFMAs later, in the shadow of the next.
+//
+// 4096 x [16384 x 2560] (256 x 256 tiles) takes 155 to 162 us, 2.1 to 2.2 PFLOP/s.
+// With parts of it left out (copies of the kernel): the MFMAs alone 110, with the
+// scaling 120, with the reads of LDS 127, with the loads 145, with the stores 160.
+// So it is bound by the matrix cores, and what is not under them is the stores of
+// 128 KB per CU and tile, which all CUs come to at about the same time: a tile's 20
+// k-tiles are too few to hide them.  4096 tokens x 8 over 128 experts of [2560 x
+// 640] (five k-tiles a tile) takes 117 to 120 us: 75, with the loads 95, with the
+// stores 118; its bytes are 82 us' worth.  No gain from wave priorities, loads into
+// L2 ahead, spread or bunched loads, later waits, workgroups that start apart,
+// other bands (gm) of tiles, or scale blocks that lie an odd number of lines apart.
 //
 // Weight rows are dealt to the MFMA's rows so that a lane holds 4 NS
 // neighbouring columns of each of its rows of y.
