@@ -265,10 +265,12 @@ def f8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
     [M, K] with fp32 scales [M, ceil(K/128)] (fmt "e4m3_g128" above; of any
     strides, but fastest as that lays them out), weights [N, K] with scales per
     128 x 128 block (quantize_f8).  Blocks are summed in fp32.  Any M and N, K up
-    to 131071; out_dtype bf16 or fp16, whose products are the matrix cores' fp8 ones (eight
-    at a time, cut to 2^-13 of the largest: 1.5e-5 of a result), or fp32, for
-    which they are exact, at half of the rate.  Code rows that do not start on 16 bytes are
-    copied first; a bias that is not fp32 is converted in every call."""
+    to 131071; out_dtype bf16 or fp16, whose products are the matrix cores' fp8
+    ones (eight at a time, cut to 2^-13 of the largest: 1.5e-5 of a result), or
+    fp32, for which they are exact, at half of the rate.  Code rows that do not
+    start on 16 bytes are copied first, and rows that do not start on a line of
+    128 take up to a fifth longer (the quantizers lay theirs on lines where that
+    adds little); a bias that is not fp32 is converted in every call."""
     return _L.host().f8_linear(xq, xs, wq, ws, bias, out_dtype)
 
 

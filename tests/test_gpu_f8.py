@@ -46,7 +46,8 @@ SIZES = [(1, 1), (3, 5), (2, 8), (5, 31), (4, 64), (3, 100), (7, 127), (2, 128),
 def test_rows(F, m, h, dt):
     x = rows(m, h, dt, m + h)
     q, s = F.quantize_q8(x.cuda(), FMT)
-    assert q.stride(0) == -(-h // 16) * 16 or m == 1
+    line = -(-h // 128) * 128                        # rows start on a line where that adds a sixteenth at most
+    assert q.stride(0) == (line if (line - h) * 16 <= h else -(-h // 16) * 16) or m == 1
     same_rows(q, s, x.float().numpy())
 
 
