@@ -290,8 +290,9 @@ Tensor codes16(const Tensor& q, const char* what, at::ScalarType type = at::kCha
       (q.stride(-1) == 1 || k == 1) && k <= ld && ld < 1 << 24 &&
       (k == up || (uint64_t)(q.storage_offset() + (e - 1) * step + (n - 1) * ld + up) <= q.storage().nbytes()))
     return q;
-  const c10::Storage whole = make({e * n * up}, {1}, at::kByte, q).storage();    // whole rows, the last too
-  const Tensor c = dims == 3 ? part(whole, 0, {e, n, k}, {n * up, up, 1}, type) : part(whole, 0, {n, k}, {up, 1}, type);
+  const int64_t to = type == at::kChar ? up : line_rows(k);
+  const c10::Storage whole = make({e * n * to}, {1}, at::kByte, q).storage();    // whole rows, the last too
+  const Tensor c = dims == 3 ? part(whole, 0, {e, n, k}, {n * to, to, 1}, type) : part(whole, 0, {n, k}, {to, 1}, type);
   c.copy_(q);
   return c;
 }

@@ -280,7 +280,8 @@ def f8_linear_experts(xq, xs, wq, ws, offsets, tokens=None, out_dtype=torch.bflo
     tokens (int32 [P]), row s of the result [P, N] is that of row tokens[s] of xq
     (the first product after expert_sort; nothing is gathered in memory);
     without, of row s (the second).  offsets is int32 [E + 1], as expert_sort
-    gives it; rows from offsets[E] on are not written.  At most 4096 experts."""
+    gives it; rows from offsets[E] on are not written.  At most 4096 experts;
+    rows that tokens pick from lie within 2^32 bytes."""
     return _L.host().f8_linear_experts(xq, xs, wq, ws, offsets, tokens, out_dtype)
 
 

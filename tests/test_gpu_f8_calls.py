@@ -7,6 +7,7 @@ import os
 import pytest
 import torch
 
+from oracle import f8 as o
 from test_gpu_experts import expert_operands, plain_experts
 from test_gpu_experts import route as host_route
 from test_gpu_f8 import FMT, exact_operands, exact_product
@@ -86,6 +87,14 @@ def test_empty_calls(F):
     assert dy.shape == (0, 8) and torch.equal(dw, torch.zeros((3, 2), device="cuda"))
     q, s = F.quantize_f8(torch.ones((0, 8), device="cuda"))
     assert q.shape == (0, 8) and s.shape == (0, 1)
+
+
+@pytest.mark.parametrize("t,k", [(30, 8), (40, 8), (128, 8), (129, 8), (1025, 4)])
+def test_sort_of_the_most_experts(F, t, k):
+    """4096 counts per wave, where those of four waves are 64 KB of LDS and of eight 128."""
+    ids = route(t, k, 4096, t, drop=0.1)
+    for got, want in zip(F.expert_sort(ids, 4096), o.sort(ids.cpu().numpy(), 4096)):
+        assert (got.cpu().numpy() == want).all()
 
 
 @pytest.mark.parametrize("t,k,experts", [(700, 8, 60), (9000, 8, 512), (1100, 2, 4096)])
@@ -184,6 +193,20 @@ def test_outputs_and_weights_past_2_32_bytes(F):
     assert torch.equal(got, F.f8_linear(aq, as_, cq, cs, out_dtype=torch.float32))
 
 
+def test_codes_that_are_copied(F):
+    """Rows, and weights of experts, that do not start on 16 bytes, or whose last row cannot be read to 16 bytes."""
+    xq, xs, wq, ws = expert_operands(90, 3, 70, 300, 9)
+    offsets, tokens, _ = F.expert_sort(route(90, 2, 3, 1), 3)
+    want = plain_experts(xq, xs, wq, ws, offsets, tokens).float()
+
+    def off(q, by):                                  # the same codes, side by side, `by` bytes into a buffer
+        b = torch.empty(q.numel() + by, dtype=torch.uint8, device="cuda")[by:].view(q.shape)
+        b.copy_(q.view(torch.uint8))
+        return b.view(q.dtype)
+    for x, w in ((xq.contiguous(), wq), (xq, wq.contiguous()), (off(xq, 5), off(wq, 3)), (off(xq, 16), off(wq, 16))):
+        assert torch.equal(F.f8_linear_experts(x, xs, w, ws, offsets, tokens, out_dtype=torch.float32), want)
+
+
 def test_a_weight_that_repeats(F):
     """One weight for all experts, expanded: its rows have a stride of 0 between experts."""
     xq, xs, wq, ws = expert_operands(300, 1, 200, 256, 4)
@@ -238,3 +261,52 @@ def test_example_gradients(F, example):
     for got, want, size, n in ((leaf[0].grad, dx, (w[..., None] * f * d64[:, None]).abs().sum(1), k + 3),
                                (leaf[1].grad, dw, (f * x[:, None] * d64[:, None]).abs().sum(2), h + 3)):
         assert ((got.double() - want).abs() <= 1.01 * n * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("t,k,experts", [(1 << 20, 1, 512), ((1 << 20) + 77, 1, 512), (300000, 7, 4096), (1000003, 4, 3)])
+def test_sort_of_several_rounds(F, t, k, experts):
+    """More pairs than the workgroups' waves count at 256 each: every wave takes several rounds."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    ids = torch.randint(-1, experts + 1, (t, k), generator=g, device="cuda")
+    offsets, tokens, slots = F.expert_sort(ids, experts)
+    flat = torch.where((ids < 0) | (ids >= experts), experts, ids).reshape(-1)
+    key, order = torch.sort(flat, stable=True)
+    n = int((key < experts).sum())
+    assert torch.equal(offsets.long(), torch.searchsorted(key, torch.arange(experts + 1, device="cuda")))
+    assert torch.equal(tokens[:n].long(), order[:n] // k) and (tokens[n:] == -1).all()
+    want = torch.full_like(flat, -1)
+    want[order[:n]] = torch.arange(n, device="cuda")
+    assert torch.equal(slots.reshape(-1).long(), want)
+
+
+def test_past_the_grids(F):
+    """More rows, pairs and blocks than a launch has workgroups: the ends of what the loops over them reach."""
+    for m, h in ((67108869, 16), (4194309, 264), (1048579, 1032)):
+        x = torch.zeros((m, h), dtype=torch.bfloat16, device="cuda")
+        x[-9:] = torch.randn((9, h), device="cuda")
+        q, s = F.quantize_q8(x, FMT)
+        q9, s9 = F.quantize_q8(x[-9:].clone(), FMT)
+        assert torch.equal(q[-9:].float(), q9.float()) and torch.equal(s[-9:], s9)
+        assert torch.equal(s[:-9].amax(), s[0, 0]) and not q[:64].float().any()
+        del x, q, s
+    w = torch.randn((1048580, 1, 8), device="cuda")
+    q, s = F.quantize_f8(w)
+    q9, s9 = F.quantize_f8(w[-9:].clone())
+    assert torch.equal(q[-9:].float(), q9.float()) and torch.equal(s[-9:], s9)
+    p = 4194309
+    y = torch.randn((p, 8), device="cuda")
+    at = torch.randperm(p, device="cuda").int()
+    assert torch.equal(F.expert_combine(y, at[:, None]), y[at.long()])
+    assert torch.equal(F.expert_rows(y, at), y[at.long()])
+    at = torch.randint(0, 1 << 20, (8388700,), device="cuda", dtype=torch.int32)
+    assert torch.equal(F.expert_rows(y[:1 << 20], at), y[at.long()])
+
+
+def test_the_most_rows(F):
+    """2^24 rows: the tallest product."""
+    xq, xs, wq, ws = exact_operands(256, 16, 16, 1)
+    rows_ = torch.arange(1 << 24, device="cuda") % 256
+    bx = xq.view(torch.uint8)[rows_].view(xq.dtype)
+    out = F.f8_linear(bx, xs[rows_], wq, ws)
+    want = exact_product(xq, xs, wq, ws).float().bfloat16()
+    assert torch.equal(out.view(-1, 256, 16), want.expand(1 << 16, -1, -1))
