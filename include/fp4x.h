@@ -345,8 +345,9 @@ int fp4x_f8_experts_form(int P, int N, int K, int E, int out_dtype);
  * the experts' products: offsets int32 [E + 1] where each expert's begin, tokens
  * int32 [T k] the token of each row (-1 behind the last), slots int32 [T, k] the
  * row of each pair (-1: none).  At most 2^30 pairs, 4096 experts.  The workspace
- * (bytes from the query, 0 up to 4096 pairs) needs no contents and is not used
- * after the call.  No counterpart in the reference. */
+ * (bytes from the query; 0 up to 2048 pairs, or 4096 of at most 2048 experts)
+ * needs no contents and is not used after the call.  No counterpart in the
+ * reference. */
 int64_t fp4x_expert_sort_workspace(int64_t T, int k, int E);
 int fp4x_expert_sort(const void* ids, int wide, int64_t row, int64_t T, int k, int E, int* offsets, int* tokens,
                      int* slots, void* workspace, int64_t workspace_bytes, void* stream);

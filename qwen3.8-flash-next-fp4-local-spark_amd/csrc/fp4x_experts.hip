@@ -39,8 +39,8 @@ static int ex_fail(const char* what, const char* why) {
 // of E counts, from L2).
 //
 // Bound by latency, not by its 24 bytes per pair: 24 pairs of 512 experts take 2.8
-// us, 32008 of 256 experts 4.8 + 7.5 in two launches, where the bytes are 0.2: a
-// kernel's start and reads that wait for each other (ids, the chunks' counts).
+// us, 32008 of 256 experts 8.7 in two launches, where the bytes are 0.2: a kernel's
+// start and reads that wait for each other (ids, the chunks' counts).
 constexpr int kSortOne = 4096, kSortChunks = 256;
 
 struct SortArgs {
@@ -177,10 +177,13 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(const SortArgs a) {
   for (int64_t s = carry + (int64_t)blockIdx.x * blockDim.x + t; s < a.P; s += (int64_t)gridDim.x * blockDim.x) a.tokens[s] = -1;
 }
 
-// Chunks of W waves; W by the pairs (few pairs: few counts to clear and to add) and by the LDS that E counts per wave take.
+// Chunks of W waves: few where few pairs leave few counts to clear and to add; 16 where one launch is enough (4800 pairs in one
+// launch of two rounds take 9.6 to 11.3 us, in two launches 7.7 to 8.8) or the chunks' counts take longer to add than the waves'
+// (320000 pairs of 256 experts 15.2 us, 16.0 with 8 waves and 21.2 with 4); 8 between (32768 of 512: 9.3; 10.9 with 16, 9.5 with 4),
+// and where 16 would not fit the LDS.
 struct SortPlan {
   int W, rounds, chunks;
-  SortPlan(int64_t P, int E) : W(P <= 256 ? 1 : P <= 1024 ? 4 : E <= 2048 ? 16 : 8), rounds(1), chunks(1) {
+  SortPlan(int64_t P, int E) : W(P <= 256 ? 1 : P <= 1024 ? 4 : E <= 2048 && (P <= kSortOne || P > 1 << 18) ? 16 : 8), rounds(1), chunks(1) {
     if (P > kSortOne || P > 256 * W) {
       rounds = (int)((P + (int64_t)kSortChunks * 256 * W - 1) / ((int64_t)kSortChunks * 256 * W));
       chunks = (int)((P + (int64_t)256 * W * rounds - 1) / ((int64_t)256 * W * rounds));
