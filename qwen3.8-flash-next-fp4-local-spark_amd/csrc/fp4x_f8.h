@@ -365,13 +365,15 @@ __global__ __launch_bounds__(64 * W, 2) void f8_ring_kernel(const F8Args a) {
 // 4096 x [16384 x 2560] (256 x 256 tiles) takes 155 to 162 us, 2.1 to 2.2 PFLOP/s.
 // With parts of it left out (copies of the kernel): the MFMAs alone 110, with the
 // scaling 120, with the reads of LDS 127, with the loads 145, with the stores 160.
-// So it is bound by the matrix cores, and what is not under them is the stores of
-// 128 KB per CU and tile, which all CUs come to at about the same time: a tile's 20
-// k-tiles are too few to hide them.  4096 tokens x 8 over 128 experts of [2560 x
-// 640] (five k-tiles a tile) takes 117 to 120 us: 75, with the loads 95, with the
-// stores 118; its bytes are 82 us' worth.  No gain from wave priorities, loads into
-// L2 ahead, spread or bunched loads, later waits, workgroups that start apart,
-// other bands (gm) of tiles, or scale blocks that lie an odd number of lines apart.
+// So it is bound by the matrix cores, and what is not under them is a tile's end
+// and start (a tile has 20 k-tiles).  4096 tokens x 8 over 128 experts of [2560 x
+// 640] (five k-tiles a tile) takes 110 us; its bytes are 78 us' worth.  A third of
+// its tiles' rows are none; MFMAs of such strips are left out, by wave and, in 256 x
+// 256 tiles, by half a wave's strips, with one wave of each half on a SIMD (whole
+// waves, both of a SIMD in one half: 116 us; strip by strip the registers spill).
+// No gain from wave priorities, loads into L2 ahead, spread or bunched loads, later
+// waits, workgroups that start apart, other bands (gm) of tiles, scale blocks an
+// odd number of lines apart, or a tile's stores under the next one's first MFMAs.
 //
 // Weight rows are dealt to the MFMA's rows so that a lane holds 4 NS
 // neighbouring columns of each of its rows of y.
@@ -509,7 +511,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
   };
 
   // ---- the products
-  const int wm = wave % WM, wn = wave / WM, i = lane & 15, g = lane >> 4, key = (i >> 1) & 7;
+  // Over experts a tile's upper rows may be all there are: with two waves to a SIMD each has one of its upper half.
+  constexpr bool DEAL = EX && C::W == 8;
+  const int wm = DEAL ? wave / WN : wave % WM, wn = DEAL ? wave % WN : wave / WM, i = lane & 15, g = lane >> 4, key = (i >> 1) & 7;
   // a lane's chunks of the first strip of x, and how far on the first one of w is
   const int c0 = (wm * 16 * MS + i) * 128 + (g ^ key) * 16, c1 = (wm * 16 * MS + i) * 128 + ((4 + g) ^ key) * 16;
   const int w_on = (BM + wn * 16 * NS - wm * 16 * MS) * 128;
@@ -534,11 +538,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
     return *reinterpret_cast<const float*>(lds + so + sx_at + 64 * s);
   };
   int ek = 0, et = 0;                              // the k-tile that is multiplied, and its tile
-  bool busy = true;                                // EX: whether the tile has rows for this wave
+  // EX: whether the tile has rows for this wave; where it owns eight strips, for how many of none, half or all.
+  constexpr bool HALVES = EX && MS >= 8;
+  std::conditional_t<HALVES, int, bool> busy = HALVES ? MS : 1;
   const auto look = [&]() __attribute__((always_inline)) {
     if constexpr (EX) {
       const F8Place ep = f8_place_of(all, min(et, tiles - 1));
-      busy = ep.m0 + wm * 16 * MS < ep.m_end;
+      const int rows = ep.m_end - ep.m0 - wm * 16 * MS;
+      if constexpr (HALVES) busy = rows <= 0 ? 0 : rows <= 8 * MS ? MS / 2 : MS;
+      else busy = ep.m0 + wm * 16 * MS < ep.m_end;
     }
   };
   const auto add = [&](int e) __attribute__((always_inline)) {   // block e of a k-tile into its sums
@@ -556,10 +564,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
   };
   // Step s of a k-tile in stage so.  In the last step `more` reads from the next stage `nx`, and `fill` issues the loads
   // of the stage that the barrier freed.  The order is pinned: an MFMA, then what does not wait for it.
-  // A wave that the tile has no rows for only takes its part in the loads.
+  // Strips that the tile has no rows for are left out, but for the wave's part in the loads.
   const auto step = [&](int s, int so, bool more, int nx, bool fill) __attribute__((always_inline)) {
     const bool end = s == MS - 1;
-    if (EX && !busy) {
+    if (EX && (HALVES && s >= MS / 2 ? busy != MS : !busy)) {
+      if (HALVES && s == MS / 2 && busy) {
+        add(s * NS - 2);
+        add(s * NS - 1);
+      }
       if (fill)
 #pragma unroll
         for (int j = 0; j < NL; ++j) load(j, so);
@@ -612,6 +624,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
     constexpr int DT = decltype(dt)::value, PER = DT == DT_F32 ? 4 : 8, NP = 4 * NS / PER;
 #pragma unroll
     for (int s = 0; s < MS; ++s) {
+      if (HALVES && s >= MS / 2 && busy != MS) break;
       uint32_t d[NP][4];
 #pragma unroll
       for (int q = 0; q < NP; ++q)
