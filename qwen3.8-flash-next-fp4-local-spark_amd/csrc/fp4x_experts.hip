@@ -204,29 +204,31 @@ static int launch_sort(const SortArgs& a, hipStream_t st) {
 
 // ------------------------------------------------------------------ rows
 // Bytes are copied as they are, 16 at a time, the last 16 of a row again where
-// its length is no multiple.  A wave takes up to kRowPart bytes of a row.
+// its length is no multiple.  A wave takes a part of a row, 4 KB at most, by C
+// loads that are on their way together.
 //
 // Experts share tokens: each row of x is read k times, by rows of the output that
-// lie far apart.  So where that is four times or more, and the output is larger
-// than the L2, an XCD (workgroups go to the eight in turn) takes the rows whose
-// tokens are in its eighth of x, which its L2 keeps, and the output passes by: for
-// each 16 rows, each XCD has a wave that copies its own of them.  32768 rows of
-// 2560 in bf16 took 48 us without this (40 with it: 188 MB at 4.7 TB/s, bound by
-// the writes), 131072 of 1024 79 (58); at two rows per token it loses (26 against
-// 33 at 8192 of 5120).
-constexpr int kRowPart = 8192;
+// lie far apart.  So where that is twice or more, and the output is larger than the
+// L2, an XCD (workgroups go to the eight in turn) takes the rows whose tokens are in
+// its eighth of x, which its L2 keeps, and the output passes by: for each kRowGroup
+// rows, each XCD has a wave that copies its own of them.  32768 rows of 4096 tokens,
+// 2560 in bf16, take 29.7 us (189 MB at 6.4 TB/s; 48 without this, 62 with stores
+// that stay in L2, 36 with groups of 8, 42 with 2), 131072 of 1024 52 (78), 16384 of
+// 8192 tokens and 5120 values 52 (57).
+constexpr int kRowPart = 4096, kRowGroup = 4;
 typedef uint32_t u32x4_b __attribute__((ext_vector_type(4), aligned(1)));
 
 struct RowsArgs {
   const uint8_t* x;  int64_t x_stride;             // bytes
   const int* tokens;
   uint8_t* out;  int64_t out_stride;
-  int T, P, parts;
+  int T, P, parts, part;                           // parts of a row, bytes of one (a multiple of 128, the last may be shorter)
   int64_t bytes;
 };
-template <bool STREAM>
+template <int C, bool STREAM>
 __device__ __forceinline__ void copy_row(const RowsArgs& a, int lane, int64_t s, int tok, int part) {
-  const int64_t b0 = (int64_t)part * kRowPart, n = min(a.bytes - b0, (int64_t)kRowPart);
+  const int64_t b0 = (int64_t)part * a.part;
+  const int n = (int)min(a.bytes - b0, (int64_t)a.part);
   const bool has = tok >= 0 && tok < a.T;
   const uint8_t* from = a.x + (int64_t)(has ? tok : 0) * a.x_stride + b0;
   uint8_t* to = a.out + s * a.out_stride + b0;
@@ -234,47 +236,59 @@ __device__ __forceinline__ void copy_row(const RowsArgs& a, int lane, int64_t s,
     if (lane < n) to[lane] = has ? from[lane] : 0;
     return;
   }
-  for (int64_t b = lane * 16; b - lane * 16 < n; b += 4096) {
-    u32x4_b v[4];
-    if (has) {
+  const int b = lane * 16;
+  u32x4_b v[C];
+  if (has) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const u32x4_b*>(from + min(b + i * 1024, n - 16));
-    } else {
+    for (int i = 0; i < C; ++i) v[i] = *reinterpret_cast<const u32x4_b*>(from + min(b + i * 1024, n - 16));
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = u32x4_b{0, 0, 0, 0};
-    }
+    for (int i = 0; i < C; ++i) v[i] = u32x4_b{0, 0, 0, 0};
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u32x4_b* p = reinterpret_cast<u32x4_b*>(to + min(b + i * 1024, n - 16));
-      if (b + i * 1024 < n) {
-        if constexpr (STREAM) __builtin_nontemporal_store(v[i], p);
-        else *p = v[i];
-      }
+  for (int i = 0; i < C; ++i) {
+    u32x4_b* p = reinterpret_cast<u32x4_b*>(to + min(b + i * 1024, n - 16));
+    if (b + i * 1024 < n) {
+      if constexpr (STREAM) __builtin_nontemporal_store(v[i], p);
+      else *p = v[i];
     }
   }
 }
+template <int C>
 __global__ __launch_bounds__(256) void expert_rows_kernel(const RowsArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * 4, items = (int64_t)a.P * a.parts;
   for (int64_t it = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); it < items; it += waves) {
     const int64_t s = it / a.parts;
-    copy_row<false>(a, lane, s, a.tokens[s], (int)(it - s * a.parts));
+    copy_row<C, false>(a, lane, s, a.tokens[s], (int)(it - s * a.parts));
   }
 }
+template <int C>
 __global__ __launch_bounds__(256) void expert_rows_large_kernel(const RowsArgs a) {
   const int lane = threadIdx.x & 63, xcd = blockIdx.x & 7;
   const int lo = (int)((int64_t)a.T * xcd >> 3), hi = (int)((int64_t)a.T * (xcd + 1) >> 3);
-  const int64_t waves = (int64_t)(gridDim.x >> 3) * 4, items = (((int64_t)a.P + 15) >> 4) * a.parts;   // (the grid is a multiple of 8)
+  const int64_t waves = (int64_t)(gridDim.x >> 3) * 4;   // (the grid is a multiple of 8)
+  const int64_t items = ((int64_t)a.P + kRowGroup - 1) / kRowGroup * a.parts;
   for (int64_t it = (int64_t)(blockIdx.x >> 3) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); it < items; it += waves) {
-    const int64_t g = it / a.parts, s = g * 16 + lane;
-    const int tok = lane < 16 && s < a.P ? a.tokens[s] : -1;
+    const int64_t g = it / a.parts, s = g * kRowGroup + lane;
+    const bool in = lane < kRowGroup && s < a.P;
+    const int tok = in ? a.tokens[s] : -1;
     const bool none = tok < 0 || tok >= a.T;       // zeros: dealt by their place
-    uint64_t mine = __ballot(lane < 16 && s < a.P && (none ? (lane & 7) == xcd : tok >= lo && tok < hi));
+    uint64_t mine = __ballot(in && (none ? ((int)s & 7) == xcd : tok >= lo && tok < hi));
     while (mine) {
       const int l = __builtin_ctzll(mine);
       mine &= mine - 1;
-      copy_row<true>(a, lane, g * 16 + l, __builtin_amdgcn_readlane(tok, l), (int)(it - g * a.parts));
+      copy_row<C, true>(a, lane, g * kRowGroup + l, __builtin_amdgcn_readlane(tok, l), (int)(it - g * a.parts));
     }
+  }
+}
+template <int C>
+static void launch_rows(const RowsArgs& a, bool large, hipStream_t st) {
+  if (large) {
+    const int64_t waves = ((int64_t)a.P + kRowGroup - 1) / kRowGroup * a.parts;   // on each XCD
+    hipLaunchKernelGGL((expert_rows_large_kernel<C>), dim3((unsigned)std::min<int64_t>((waves + 3) / 4, 1 << 17) * 8), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((expert_rows_kernel<C>), dim3((unsigned)std::min<int64_t>(((int64_t)a.P * a.parts + 3) / 4, 1 << 20)), dim3(256), 0, st, a);
   }
 }
 
@@ -566,15 +580,15 @@ int fp4x_expert_rows(const void* x, int64_t x_stride, int elem, int T, const int
   if (x_stride < 0 || (P > 1 && out_stride < H)) return ex_fail(what, "output rows overlap, or a stride is negative");
   const int64_t bytes = (int64_t)H * elem;
   const int64_t parts = (bytes + kRowPart - 1) / kRowPart;
+  const int part = (int)(((bytes + parts - 1) / parts + 127) & -128);
   const RowsArgs a{static_cast<const uint8_t*>(x), x_stride * elem, tokens, static_cast<uint8_t*>(out), out_stride * elem,
-                   T, P, (int)parts, bytes};
+                   T, P, (int)parts, part, bytes};
   hipStream_t st = (hipStream_t)stream;
-  if (P / 4 >= T && T >= 8 && P * bytes > 32 << 20) {
-    const dim3 grid((unsigned)std::min<int64_t>((((int64_t)P + 15) / 16 * parts + 3) / 4, 1 << 17) * 8);
-    hipLaunchKernelGGL(expert_rows_large_kernel, grid, dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL(expert_rows_kernel, dim3((unsigned)std::min<int64_t>((P * parts + 3) / 4, 1 << 20)), dim3(256), 0, st, a);
-  }
+  const bool large = P / 2 >= T && T >= 8 && P * bytes > 32 << 20;
+  if (part <= 1024) launch_rows<1>(a, large, st);
+  else if (part <= 2048) launch_rows<2>(a, large, st);
+  else if (part <= 3 * 1024) launch_rows<3>(a, large, st);
+  else launch_rows<4>(a, large, st);
   return check_launch(what);
 }
 

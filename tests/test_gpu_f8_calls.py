@@ -310,3 +310,23 @@ def test_the_most_rows(F):
     out = F.f8_linear(bx, xs[rows_], wq, ws)
     want = exact_product(xq, xs, wq, ws).float().bfloat16()
     assert torch.equal(out.view(-1, 256, 16), want.expand(1 << 16, -1, -1))
+
+
+@pytest.mark.parametrize("t,k,h,dt", [(4001, 8, 2560, torch.bfloat16), (3000, 6, 2571, torch.float32), (9000, 4, 1000, torch.float16),
+                                      (70000, 3, 255, torch.uint8), (2500, 8, 1500, torch.bfloat16), (5000, 2, 4097, torch.bfloat16),
+                                      (9, 900, 4199, torch.int8), (2100, 4, 1030, torch.int32), (4000000, 5, 3, torch.bfloat16)])
+def test_large_rows(F, t, k, h, dt):
+    """Rows of tokens that share them, more than the L2 holds: every length of a part, rows that start anywhere, a third without a token."""
+    assert t * k * h * dt.itemsize > 32 << 20
+    g = torch.Generator(device="cuda").manual_seed(h)
+    bits = torch.randint(0, 256, (t * (h + 1) * dt.itemsize,), generator=g, device="cuda", dtype=torch.uint8)
+    x = bits.view(dt).view(t, h + 1)[:, 1:]
+    tokens = torch.randint(-t // 2, t, (t * k,), generator=g, device="cuda", dtype=torch.int32)
+    tokens[5::7] = t                                 # (behind the last)
+    got = F.expert_rows(x, tokens)
+    one = {1: torch.uint8, 2: torch.int16, 4: torch.int32}[dt.itemsize]
+    x, got = x.contiguous().view(one), got.view(one)
+    for part in range(0, t * k, 1 << 22):
+        tk = tokens[part:part + (1 << 22)].long()
+        has = ((tk >= 0) & (tk < t))[:, None]
+        assert torch.equal(got[part:part + (1 << 22)], torch.where(has, x[tk.clamp(0, t - 1)], torch.zeros((), dtype=one, device="cuda")))
