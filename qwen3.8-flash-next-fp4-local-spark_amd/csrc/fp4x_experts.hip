@@ -314,18 +314,24 @@ template <int DT> struct Vec8 {
     else return f16_to_f32((uint16_t)(j & 1 ? d >> 16 : d));
   }
 };
-template <int DT>
+// Eight values; STREAM: they pass by the L2.
+template <bool STREAM>
+__device__ __forceinline__ void put4(u32x4_e* p, u32x4_e v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <int DT, bool STREAM>
 __device__ __forceinline__ void put8(void* p, int64_t i, const float (&f)[8]) {
   if constexpr (DT == DT_F32) {
     u32x4_e* g = reinterpret_cast<u32x4_e*>(static_cast<float*>(p) + i);
-    g[0] = u32x4_e{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
-    g[1] = u32x4_e{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
+    put4<STREAM>(g, u32x4_e{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])});
+    put4<STREAM>(g + 1, u32x4_e{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])});
   } else {
     uint32_t d[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       d[j] = DT == DT_BF16 ? pack_bf16x2(f[2 * j], f[2 * j + 1]) : pack_f16x2(f[2 * j], f[2 * j + 1]);
-    *reinterpret_cast<u32x4_e*>(static_cast<uint16_t*>(p) + i) = u32x4_e{d[0], d[1], d[2], d[3]};
+    put4<STREAM>(reinterpret_cast<u32x4_e*>(static_cast<uint16_t*>(p) + i), u32x4_e{d[0], d[1], d[2], d[3]});
   }
 }
 template <int DT>
@@ -349,8 +355,8 @@ struct CombineArgs {
 // A wave takes 512 values of a token, eight per lane, and its k rows B at a time, whose loads are on their way together (B 8
 // for two rows left registers for 5 waves per SIMD: 20000 tokens of 2 rows of 700 took 34 us).  The last lanes of a row are
 // moved back to end at H.  Sums are fp32 by fma, rounded once.  Bound by the reads: 4096 tokens of 8 rows of 2560 in bf16,
-// 189 MB, take 42 us (4.5 TB/s); 3 tokens 3.0 (latency).
-template <int DT, int B>
+// 189 MB, take 40 us (4.8 TB/s); 3 tokens 3.0 (latency).
+template <int DT, int B, bool STREAM>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const CombineArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * 4, items = (int64_t)a.T * a.parts;
@@ -389,16 +395,25 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const CombineArgs a
 #pragma unroll
           for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w[j], v[j].get(i), acc[i]);
     }
-    if (h0 < a.H) put8<DT>(a.out, t * a.out_stride + h, acc);
+    if (h0 < a.H) put8<DT, STREAM>(a.out, t * a.out_stride + h, acc);
   }
 }
 
+// Where y does not stay in the 32 MB of the XCDs' L2, neither do the results: they would push out what other waves are about
+// to read (4096 tokens of 8 rows of 2560 in bf16: the sum 43.0 us so, 39.7 with stores that pass by; the gradient 78 and 76).
+static bool ex_streams(int64_t P, int64_t H, int dt) { return P * H * (dt == DT_F32 ? 4 : 2) > 32 << 20; }
+
+template <int DT, bool STREAM>
+static void launch_combine_as(const CombineArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.T * a.parts + 3) / 4, 1 << 20));
+  if (a.k <= 2) hipLaunchKernelGGL((expert_combine_kernel<DT, 2, STREAM>), grid, dim3(256), 0, st, a);
+  else if (a.k <= 4) hipLaunchKernelGGL((expert_combine_kernel<DT, 4, STREAM>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((expert_combine_kernel<DT, 8, STREAM>), grid, dim3(256), 0, st, a);
+}
 template <int DT>
 static void launch_combine(const CombineArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.T * a.parts + 3) / 4, 1 << 20));
-  if (a.k <= 2) hipLaunchKernelGGL((expert_combine_kernel<DT, 2>), grid, dim3(256), 0, st, a);
-  else if (a.k <= 4) hipLaunchKernelGGL((expert_combine_kernel<DT, 4>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((expert_combine_kernel<DT, 8>), grid, dim3(256), 0, st, a);
+  if (ex_streams(a.P, a.H, DT)) launch_combine_as<DT, true>(a, st);
+  else launch_combine_as<DT, false>(a, st);
 }
 
 // ------------------------------------------------------------------ its gradient
@@ -435,7 +450,7 @@ __device__ __forceinline__ float wave_total(float v) {
 // order, and the waves' are added in theirs.  Workgroups past the tokens clear the
 // rows that no pair has.  Bound by memory: 4096 tokens of 8 rows of 2560 in bf16,
 // 357 MB, take 70 us (5.1 TB/s, a large copy's rate).
-template <int DT, int C>
+template <int DT, int C, bool STREAM>
 __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
   __shared__ float sum[16][kGradTop];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), W = blockDim.x >> 6;
@@ -503,7 +518,7 @@ __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
             g[i] = w[j] * d[c].get(i);
             if (in[c] && i >= dup) dot[j] = __builtin_fmaf(d[c].get(i), v[j][c].get(i), dot[j]);
           }
-          if (in[c]) put8<DT>(a.dy, s[j] * a.dy_stride + h[c], g);
+          if (in[c]) put8<DT, STREAM>(a.dy, s[j] * a.dy_stride + h[c], g);
         }
     }
 #pragma unroll
@@ -520,17 +535,21 @@ __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
   }
 }
 
-template <int DT>
-static int launch_grad(const GradArgs& a, hipStream_t st) {
+template <int DT, bool STREAM>
+static int launch_grad_as(const GradArgs& a, hipStream_t st) {
   const int chunks = (a.H + 7) / 8, C = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 4;
   const int threads = std::min(1024, ((chunks + C - 1) / C + 63) / 64 * 64);
   const int64_t groups = a.T + (a.P + (int64_t)kGradTail - 1) / kGradTail;
   if (groups * threads > (int64_t)UINT32_MAX) return ex_fail("expert_combine_grad", "tokens times the lanes of a row pass 2^32");
   const dim3 grid((unsigned)groups);
-  if (C == 1) hipLaunchKernelGGL((expert_grad_kernel<DT, 1>), grid, dim3(threads), 0, st, a);
-  else if (C == 2) hipLaunchKernelGGL((expert_grad_kernel<DT, 2>), grid, dim3(threads), 0, st, a);
-  else hipLaunchKernelGGL((expert_grad_kernel<DT, 4>), grid, dim3(threads), 0, st, a);
+  if (C == 1) hipLaunchKernelGGL((expert_grad_kernel<DT, 1, STREAM>), grid, dim3(threads), 0, st, a);
+  else if (C == 2) hipLaunchKernelGGL((expert_grad_kernel<DT, 2, STREAM>), grid, dim3(threads), 0, st, a);
+  else hipLaunchKernelGGL((expert_grad_kernel<DT, 4, STREAM>), grid, dim3(threads), 0, st, a);
   return check_launch("expert_combine_grad");
+}
+template <int DT>
+static int launch_grad(const GradArgs& a, hipStream_t st) {
+  return ex_streams(a.P, a.H, DT) ? launch_grad_as<DT, true>(a, st) : launch_grad_as<DT, false>(a, st);
 }
 
 static bool ex_dt(int dt) { return dt == DT_BF16 || dt == DT_F32 || dt == DT_F16; }

@@ -330,3 +330,33 @@ def test_large_rows(F, t, k, h, dt):
         tk = tokens[part:part + (1 << 22)].long()
         has = ((tk >= 0) & (tk < t))[:, None]
         assert torch.equal(got[part:part + (1 << 22)], torch.where(has, x[tk.clamp(0, t - 1)], torch.zeros((), dtype=one, device="cuda")))
+
+
+@pytest.mark.parametrize("t,k,h,dt", [(4001, 8, 1290, torch.bfloat16), (9000, 2, 1001, torch.float32), (3000, 4, 3333, torch.float16),
+                                      (900, 3, 17000, torch.bfloat16)])
+def test_large_sums_and_gradients(F, t, k, h, dt):
+    """More rows than the L2 holds, some pairs dropped: against fp64, each sum's terms and its rounding off by half a step at most."""
+    assert t * k * h * dt.itemsize > 32 << 20
+    ids = route(t, k, 24, h, drop=0.1)
+    _, tokens, slots = F.expert_sort(ids, 24)
+    y, d, w = torch.randn((t * k, h), device="cuda").to(dt), torch.randn((t, h), device="cuda").to(dt), torch.rand((t, k), device="cuda")
+    out = F.expert_combine(y, slots, w)
+    dy, dw = F.expert_combine_grad(d, y, slots, w, tokens)
+    has, at = slots >= 0, slots.clamp_min(0).long()
+    half = torch.finfo(dt).eps / 2
+    tiny = 2.0 ** -25 if dt == torch.float16 else 0.0   # half of fp16's least step
+    for t0 in range(0, t, 500):
+        p = slice(t0, t0 + 500)
+        rows_ = torch.where(has[p, :, None], y[at[p]].double(), 0.0)
+        terms = rows_ * w[p, :, None].double()
+        err = (k + 1) * 2.0 ** -24 * terms.abs().sum(1)
+        want = terms.sum(1)
+        assert ((out[p].double() - want).abs() <= err + half * (want.abs() + err) + tiny).all()
+        terms = rows_ * d[p, None].double()
+        assert ((dw[p].double() - terms.sum(2)).abs() <= (h + 1) * 2.0 ** -24 * terms.abs().sum(2)).all()
+        # one rounding from the product, or two by way of fp32 (2^-24, then half a step of what that gives)
+        want = torch.where(has[p, :, None], w[p, :, None].double() * d[p, None].double(), 0.0)
+        got = torch.where(has[p, :, None], dy[at[p]].double(), 0.0)
+        assert ((got - want).abs() <= (half + 2.0 ** -23) * want.abs() + tiny).all()
+    n = int(has.sum())
+    assert not dy[n:].any()
