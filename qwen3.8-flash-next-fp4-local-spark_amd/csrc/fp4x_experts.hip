@@ -194,7 +194,7 @@ template <int W>
 static int launch_sort(const SortArgs& a, hipStream_t st) {
   const int lds = W * a.E * (int)sizeof(int);
   const dim3 grid(a.chunks), threads(std::max(64 * W, std::min(1024, (a.E + 63) / 64 * 64)));
-  if (lds >= 64 * 1024)                            // with the 64 bytes of wave_total
+  if (lds + 16 * (int)sizeof(int) > 64 * 1024)     // sort_place's wave_total is beside it
     for (const void* f : {reinterpret_cast<const void*>(sort_count_kernel<W>), reinterpret_cast<const void*>(sort_place_kernel<W>)})
       if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return check_launch("expert_sort");
   if (a.chunks > 1) hipLaunchKernelGGL((sort_count_kernel<W>), grid, threads, lds, st, a);
