@@ -312,7 +312,9 @@ int fp4x_quantize_f8(const void* w, int64_t w_row, int64_t w_expert, int dtype, 
  * ws[n / 128, b]) + bias[n]), b the blocks of 128 values of K: e4m3 codes, a
  * block's sum from the matrix cores, scaled and added in fp32.  For bf16 and fp16
  * outputs the products are the fp8 instruction's, which adds eight at a time, cut
- * to 2^-13 of the power of two of the largest; for fp32 outputs they are exact.
+ * towards zero to 2^-13 of the power of two of the largest: at worst 8.5e-4 of the
+ * largest product of each eight, which is no bound relative to a result in which
+ * larger products cancel; for fp32 outputs they are exact.
  * xs fp32 at xs[m * xs_row + b * xs_block] (FP4X_Q8_E4M3_G128: xs_row 1, xs_block
  * M; reads of neighbouring rows are then one line), ws fp32 [ceil(N / 128),
  * ceil(K / 128)], bias fp32 [N] or NULL.  Code rows start on 16 bytes (strides a

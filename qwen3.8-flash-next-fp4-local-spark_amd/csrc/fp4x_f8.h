@@ -7,9 +7,13 @@
 //
 // That instruction adds eight neighbouring products at a time, each cut to 2^-13
 // of the power of two of the largest (measured; v_mfma_f32_16x16x32_fp8_fp8 does
-// the same): 1.5e-5 of a block's sum of normal values, a thirtieth of fp16's half
-// step.  For fp32 outputs (B16) both operands are turned into bf16, which
-// holds every e4m3 value, and multiplied exactly, at half of the rate.
+// the same).  On average over normal values that is 1.5e-5 of a block's sum.  At
+// worst it is 7 2^-13 = 8.5e-4 of the largest product of each eight: of the sum of
+// magnitudes, so there is no bound relative to a result that cancels, and more
+// than half a step of fp16 (4.9e-4; bf16 3.9e-3).  16-bit outputs take it all the
+// same, since codes of e4m3 are themselves off by up to 2^-4 and exact products
+// run at half of the rate.  For fp32 outputs (B16) both operands are turned into
+// bf16, which holds every e4m3 value, and multiplied exactly.
 //
 // The same over experts: rows [off[e], off[e + 1]) of the output are products
 // with expert e's weight, their rows of x picked by an index or lying in order.

@@ -266,8 +266,11 @@ def f8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
     strides, but fastest as that lays them out), weights [N, K] with scales per
     128 x 128 block (quantize_f8).  Blocks are summed in fp32.  Any M and N, K up
     to 131071; out_dtype bf16 or fp16, whose products are the matrix cores' fp8
-    ones (eight at a time, cut to 2^-13 of the largest: 1.5e-5 of a result), or
-    fp32, for which they are exact, at half of the rate.  Code rows that do not
+    ones, or fp32, for which they are exact, at half of the rate.  The fp8 ones are
+    added eight at a time, each cut towards zero to 2^-13 of the largest: 1.5e-5 of
+    a sum of normal values, at worst 8.5e-4 of the largest product of each eight
+    (more than half a step of fp16, and not relative to a result in which larger
+    products cancel; cast an fp32 result where that counts).  Code rows that do not
     start on 16 bytes are copied first, and rows that do not start on a line of
     128 take up to a fifth longer (the quantizers lay theirs on lines where that
     adds little); a bias that is not fp32 is converted in every call."""
