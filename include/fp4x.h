@@ -360,7 +360,7 @@ int fp4x_expert_rows(const void* x, int64_t x_stride, int elem, int T, const int
                      int64_t out_stride, void* stream);
 /* out[t] = sum_j w[t, j] y[slots[t, j]] in fp32, j in order (w NULL: ones); pairs
  * whose slot is no row of y [P, H] are left out and their rows not read.  out has
- * y's dtype, w [T, k] contiguous in one of its own. */
+ * y's dtype, w [T, k] contiguous in one of its own.  k and H go to 2^31 - 512. */
 int fp4x_expert_combine(const void* y, int64_t y_stride, int dtype, int P, const int* slots, const void* w, int w_dtype,
                         void* out, int64_t out_stride, int T, int k, int H, void* stream);
 /* Its gradients: dy[slots[t, j]] = w[t, j] dout[t], zeros in the rows s whose

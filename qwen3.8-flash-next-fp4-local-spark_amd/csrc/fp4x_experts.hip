@@ -14,6 +14,7 @@
 // and the gradient of the rows is the combine without weights.  No atomic decides
 // an order: every result is the same in every run.
 #include <algorithm>
+#include <climits>
 #include <string>
 
 #include "fp4x_f8.h"
@@ -616,7 +617,9 @@ int fp4x_expert_combine(const void* y, int64_t y_stride, int dtype, int P, const
                         void* out, int64_t out_stride, int T, int k, int H, void* stream) {
   const char* what = "expert_combine";
   if (!ex_dt(dtype) || (w && !ex_dt(w_dtype))) return ex_fail(what, "rows and weights are bf16, fp16 or fp32");
-  if (T < 0 || k < 1 || P < 0 || H < 1) return ex_fail(what, "need T and P >= 0, k and H >= 1");
+  // a step of the loops over k and over a row's parts stays within an int
+  constexpr int kMost = INT_MAX - 511;
+  if (T < 0 || k < 1 || P < 0 || H < 1 || k > kMost || H > kMost) return ex_fail(what, "need T and P >= 0, k and H from 1 to 2^31 - 512");
   if (T == 0) return FP4X_OK;
   if ((!y && P) || !slots || !out || !al4(slots) || !ex_al(y, dtype) || !ex_al(out, dtype) || (w && !ex_al(w, w_dtype)))
     return ex_fail(what, "null tensor, or one that is not aligned to its element");
