@@ -205,10 +205,11 @@ __device__ __forceinline__ void f8_store4(const F8Args& a, int64_t m, int n, con
 
 // 16 bytes of the output.  One that is larger than the 32 MB of the XCDs' L2 passes by it: it would push out the rows of x
 // and w that the next tiles share (4096 x [16384 x 2560] took 175 us so, 163 with these stores).  Below that the next
-// launch finds its input in the caches.
+// launch finds its input in the caches.  The store is asm because the compiler merges the two into a plain one; so it brings the two
+// wait states that lie between a store of more than 64 bits and the next VALU write of its data (the compiler sees no store here).
 template <class V>
 __device__ __forceinline__ void f8_put(V* at, V v, int stream) {
-  if (stream) asm volatile("global_store_dwordx4 %0, %1, off nt" ::"v"(at), "v"(v) : "memory");   // (two plain stores would be merged)
+  if (stream) asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 1" ::"v"(at), "v"(v) : "memory");
   else *at = v;
 }
 
