@@ -364,8 +364,10 @@ int fp4x_expert_rows(const void* x, int64_t x_stride, int elem, int T, const int
 int fp4x_expert_combine(const void* y, int64_t y_stride, int dtype, int P, const int* slots, const void* w, int w_dtype,
                         void* out, int64_t out_stride, int T, int k, int H, void* stream);
 /* Its gradients: dy[slots[t, j]] = w[t, j] dout[t], zeros in the rows s whose
- * tokens[s] is no token; dw[t, j] = dout[t] . y[slots[t, j]] (0 without a row).
- * No two slots are one row.  dy has y's dtype and shares no memory with anything
+ * tokens[s] is no token or a token that has no slot s; dw[t, j] = dout[t] .
+ * y[slots[t, j]] (0 without a row).  tokens and slots are one fp4x_expert_sort's,
+ * whose slots may have been set to -1 since; no two slots are one row.  dy has y's
+ * dtype and shares no memory with anything
  * else, dw has w's.  k <= 128, H <= 32768; tokens times the lanes of a row (H / 8
  * in whole 64s, up to 1024) stay below 2^32. */
 int fp4x_expert_combine_grad(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int dtype, int P,

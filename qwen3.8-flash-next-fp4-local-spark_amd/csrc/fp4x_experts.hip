@@ -418,7 +418,7 @@ static void launch_combine(const CombineArgs& a, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------ its gradient
-constexpr int kGradTop = 128, kGradTail = 64;      // pairs per token; rows that a workgroup of the second role looks at
+constexpr int kGradTop = 128, kGradTail = 64;      // pairs per token; rows that a workgroup of the second role looks at, one per lane
 
 struct GradArgs {
   const void* d;  int64_t d_stride;                // dout
@@ -449,18 +449,37 @@ __device__ __forceinline__ float wave_total(float v) {
 // eight values per lane, while its k rows of y go by, so that y is read and dy
 // written once for both gradients.  A wave's sum of the products has a fixed
 // order, and the waves' are added in theirs.  Workgroups past the tokens clear the
-// rows that no pair has.  Bound by memory: 4096 tokens of 8 rows of 2560 in bf16,
-// 357 MB, take 62 us after the sum of the same y and 76 over three sets of rows
-// in turn (5.8 and 4.7 TB/s; a large copy 5.1).
+// rows that no pair has: those whose token is none, or has no slot that is the row.
+// A lane looks through the slots of one row's token, so 64 rows are known after a
+// few loads on their way together (4096 tokens of 8 rows of 2560 take 74 us, by the
+// tokens alone and one row after the other 77; 100 rows of 512 191 and 181, for the
+// slots' bytes, and 200 with those dealt over a wave's lanes).  Bound by memory:
+// 4096 tokens of 8 rows of 2560 in bf16, 357 MB, take 62 us after the sum of the
+// same y and 74 over three sets of rows in turn (5.8 and 4.8 TB/s; a large copy 5.1).
+// Where pairs are dropped, rows are cleared in more time than their bytes take, one
+// after the other and an element per lane: half of the pairs 74 us, seven eighths 57
+// (their bytes 54 and 41).
 template <int DT, int C, bool STREAM>
 __global__ __launch_bounds__(1024) void expert_grad_kernel(const GradArgs a) {
   __shared__ float sum[16][kGradTop];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), W = blockDim.x >> 6;
   if ((int)blockIdx.x >= a.T) {
-    const int64_t s0 = (int64_t)(blockIdx.x - a.T) * kGradTail, s1 = min(s0 + kGradTail, (int64_t)a.P);
-    for (int64_t s = s0; s < s1; ++s) {
-      const int tok = a.tokens[s];
-      if (tok >= 0 && tok < a.T) continue;
+    __shared__ uint64_t none_of;
+    static_assert(kGradTail == 64, "a lane per row");
+    const int64_t s0 = (int64_t)(blockIdx.x - a.T) * kGradTail;
+    if (wave == 0) {
+      const int64_t s = s0 + lane;
+      const int tok = s < a.P ? a.tokens[s] : -1;
+      bool none = s < a.P;
+      if (tok >= 0 && tok < a.T)                   // a pair may have been taken out after the sort: its slot is -1
+#pragma unroll 8
+        for (int j = 0; j < a.k; ++j) none &= a.slots[(int64_t)tok * a.k + j] != (int)s;
+      const uint64_t rows = __ballot(none);
+      if (lane == 0) none_of = rows;
+    }
+    __syncthreads();
+    for (uint64_t rows = none_of; rows; rows &= rows - 1) {
+      const int64_t s = s0 + __builtin_ctzll(rows);
       for (int h = t; h < a.H; h += blockDim.x) store_out(a.dy, s * a.dy_stride + h, DT, 0.0f);
     }
     return;

@@ -315,8 +315,10 @@ def expert_combine(y, slots, weights=None):
 def expert_combine_grad(dout, y, slots, weights, tokens):
     """The gradients (dy, dweights) of expert_combine for dout [T, H] of y's type:
     dy[slots[t, j]] = weights[t, j] * dout[t] and zeros in rows without a token,
-    dweights[t, j] = dout[t] . y[slots[t, j]], 0 without a row.  tokens is
-    expert_sort's: no two slots are one row.  k <= 128, H <= 32768."""
+    dweights[t, j] = dout[t] . y[slots[t, j]], 0 without a row.  tokens and slots are
+    one expert_sort's; a pair whose slot was set to -1 since (an expert that is full)
+    leaves zeros in its row.  Where two slots are one row, that row of dy is not
+    defined.  k <= 128, H <= 32768."""
     return _L.host().expert_combine_grad(dout, y, slots, weights, tokens)
 
 
