@@ -40,8 +40,11 @@ static int ex_fail(const char* what, const char* why) {
 // of E counts, from L2).
 //
 // Bound by latency, not by its 24 bytes per pair: 24 pairs of 512 experts take 2.8
-// us, 32008 of 256 experts 8.7 in two launches, where the bytes are 0.2: a kernel's
-// start and reads that wait for each other (ids, the chunks' counts).
+// us, 32008 of 256 experts 9.3 to 10.5 in two launches (in a trace 3.8 + 6.0 at the
+// least), where the bytes are 0.2: a kernel's start and reads that wait for each
+// other (ids, the chunks' counts).  Every workgroup reads all chunks' counts, 256 E at
+// the most: 2^20 pairs take 26 us with 512 experts and 75 with 4096, where that is 1
+// GB from the L2 and the pairs' bytes are 5 us' worth.
 constexpr int kSortOne = 4096, kSortChunks = 256;
 
 struct SortArgs {
@@ -213,9 +216,9 @@ static int launch_sort(const SortArgs& a, hipStream_t st) {
 // L2, an XCD (workgroups go to the eight in turn) takes the rows whose tokens are in
 // its eighth of x, which its L2 keeps, and the output passes by: for each kRowGroup
 // rows, each XCD has a wave that copies its own of them.  32768 rows of 4096 tokens,
-// 2560 in bf16, take 29.7 us (189 MB at 6.4 TB/s; 48 without this, 62 with stores
-// that stay in L2, 36 with groups of 8, 42 with 2), 131072 of 1024 52 (78), 16384 of
-// 8192 tokens and 5120 values 52 (57).
+// 2560 in bf16, take 29.5 to 30 us over three inputs in turn (189 MB at 6.3 TB/s; 27
+// on one input; 48 without this, 62 with stores that stay in L2, 36 with groups of 8,
+// 42 with 2), 131072 of 1024 52 (78), 16384 of 8192 tokens and 5120 values 52 (57).
 constexpr int kRowPart = 4096, kRowGroup = 4;
 typedef uint32_t u32x4_b __attribute__((ext_vector_type(4), aligned(1)));
 
@@ -401,7 +404,8 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const CombineArgs a
 }
 
 // Where y does not stay in the 32 MB of the XCDs' L2, neither do the results: they would push out what other waves are about
-// to read (4096 tokens of 8 rows of 2560 in bf16: the sum 43.0 us so, 39.7 with stores that pass by; the gradient 78 and 76).
+// to read (4096 tokens of 8 rows of 2560 in bf16: the sum 43.0 us so, 39.7 with stores that pass by; the gradient 78 and
+// 76, when its workgroups that clear rows took 3 us more).
 static bool ex_streams(int64_t P, int64_t H, int dt) { return P * H * (dt == DT_F32 ? 4 : 2) > 32 << 20; }
 
 template <int DT, bool STREAM>
@@ -454,8 +458,8 @@ __device__ __forceinline__ float wave_total(float v) {
 // few loads on their way together (4096 tokens of 8 rows of 2560 take 74 us, by the
 // tokens alone and one row after the other 77; 100 rows of 512 191 and 181, for the
 // slots' bytes, and 200 with those dealt over a wave's lanes).  Bound by memory:
-// 4096 tokens of 8 rows of 2560 in bf16, 357 MB, take 62 us after the sum of the
-// same y and 74 over three sets of rows in turn (5.8 and 4.8 TB/s; a large copy 5.1).
+// 4096 tokens of 8 rows of 2560 in bf16, 357 MB, take 57 us after the sum of the
+// same y and 74 over three sets of rows in turn (6.3 and 4.8 TB/s; a large copy 5.1).
 // Where pairs are dropped, rows are cleared in more time than their bytes take, one
 // after the other and an element per lane: half of the pairs 74 us, seven eighths 57
 // (their bytes 54 and 41).

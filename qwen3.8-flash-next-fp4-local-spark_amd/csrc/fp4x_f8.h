@@ -367,15 +367,18 @@ __global__ __launch_bounds__(64 * W, 2) void f8_ring_kernel(const F8Args a) {
 // first of the next k-tile and its rows of w, each once its last MFMA is issued.
 // A block's sum is scaled and added two MFMAs later, in the shadow of the next.
 //
-// 4096 x [16384 x 2560] (256 x 256 tiles) takes 155 to 162 us, 2.1 to 2.2 PFLOP/s.
+// 4096 x [16384 x 2560] (256 x 256 tiles) takes 155 to 165 us in calls in a row,
+// 2.1 to 2.2 PFLOP/s (158 to 193 in a trace).
 // With parts of it left out (copies of the kernel): the MFMAs alone 110, with the
 // scaling 120, with the reads of LDS 127, with the loads 145, with the stores 160.
 // So it is bound by the matrix cores, and what is not under them is a tile's end
 // and start (a tile has 20 k-tiles).  4096 tokens x 8 over 128 experts of [2560 x
-// 640] (five k-tiles a tile) takes 110 us; its bytes are 78 us' worth.  A third of
+// 640] (five k-tiles a tile) takes 98 to 99 us on one input and 110 to 117 where
+// inputs change (115 to 124 in a trace); its bytes are 78 us' worth.  A third of
 // its tiles' rows are none; MFMAs of such strips are left out, by wave and, in 256 x
 // 256 tiles, by half a wave's strips, with one wave of each half on a SIMD (whole
-// waves, both of a SIMD in one half: 116 us; strip by strip the registers spill).
+// waves, both of a SIMD in one half: 116 us beside 110; strip by strip the registers
+// spill).
 // No gain from wave priorities, loads into L2 ahead, spread or bunched loads, later
 // waits, workgroups that start apart, other bands (gm) of tiles, scale blocks an
 // odd number of lines apart, or a tile's stores under the next one's first MFMAs.
@@ -624,7 +627,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_tile_kernel(const F8Args a
   int drain = 0;
   // A lane's 4 NS columns of a row are NP pieces of 16 bytes.  The four lanes of a row exchange theirs (rows of 16 lanes,
   // then halves of the wave), so that a store would write 64 bytes of each of 16 rows, and then the halves of 8 rows: a
-  // store writes whole lines of 8 rows (NP 1: 64 bytes of 16).
+  // store writes whole lines of 8 rows where those start on one (NP 1: 64 bytes of 16).
   const auto put = [&](auto dt, int l, const F8Place& ep, int n0, const float (&bs)[4 * NS]) __attribute__((always_inline)) {
     constexpr int DT = decltype(dt)::value, PER = DT == DT_F32 ? 4 : 8, NP = 4 * NS / PER;
 #pragma unroll

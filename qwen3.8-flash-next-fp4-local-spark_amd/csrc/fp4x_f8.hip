@@ -22,9 +22,11 @@ constexpr F8Form kF8Shape[kF8Forms] = {{16, 16, 2, 1, 2},   {16, 32, 2, 1, 3},  
 
 // Forms are ranked by a + n (b + d k): n tiles fall to a CU, each with k = ceil(K / 128) k-tiles, and the one with the least
 // is taken.  a, b and d are fitted to 1,000 sizes (1 to 8192 rows, 16 to 18000 columns, K from 64 to 10240; 1 to 512 experts;
-// most drawn evenly over their logarithms, weights from HBM; profiles/f8_forms.txt), so that the form taken is near the
-// fastest: on average 0.5% slower (products, 16-bit outputs; 11% at most), 0.8% (fp32 outputs; 22%), 1.3% and 1.1% (over
-// experts; 23% and 14%).  Their sums are no times: only their order counts.
+// most drawn evenly over their logarithms, weights from HBM), so that the form taken is near the fastest.  The fit is of the
+// kernels before code rows started on lines and before 256 x 256 tiles over experts left out halves of their strips; over the
+// 997 sizes that profiles/f8_forms.txt lists with the kernels as they are, the form taken is on average 0.4% slower (products,
+// 16-bit outputs; 15% at most), 0.8% (fp32 outputs; 22%), 1.4% and 1.1% (over experts; 32% and 16%).  The estimate's values
+// are no times: only their order counts.
 struct F8Cost { float a, b, d; };
 constexpr F8Cost kF8Cost[2][2][kF8Forms] = {
     {{{0.84f, 0.852f, 0.0396f}, {1.12f, 0.858f, 0.0582f}, {1.28f, 1.022f, 0.0661f}, {0.80f, 3.811f, 0.0805f},
@@ -59,7 +61,10 @@ static int f8_best(int ex, bool b16, int N, int K, Rows rows) {
 static int choose_f8(int M, int N, int K, bool b16) {
   return f8_best(0, b16, N, K, [&](int bm) { return (float)((M + bm - 1) / bm); });
 }
-// As if the pairs fell on the experts evenly: so many are hit, and a hit one's rows end half-way through a tile.
+// As if the pairs fell on the experts evenly: so many are hit, and a hit one's rows end half-way through a tile.  M is all that
+// is known here: where part of the pairs have no expert (another rank's), it counts them too, and the tiles are too tall for the
+// rows that are left.  4096 tokens x 8 over 512 experts of [1280 x 2560], 64 of them here (3,600 to 5,800 rows kept): 78 us with the
+// whole list of tokens, 49 with the list cut to the rows kept, whose number the host must know for that.
 static int choose_f8_experts(int M, int N, int K, int E, bool b16) {
   const float hit = E == 1 ? 1.0f : (float)E * (1.0f - std::exp(-(float)M / (float)E)), mean = (float)M / hit;
   return f8_best(1, b16, N, K, [&](int bm) { return hit * (mean <= 0.7f * (float)bm ? 1.0f : mean / (float)bm + 0.5f); });

@@ -9,9 +9,11 @@ namespace fp4x {
 // Lanes and chunks per lane as the other formats have them (launch_row_q8), but
 // where that leaves a quarter of them or more without values: blocks need no more
 // than 16 lanes, so rows may share a wave, and the fewest idle of 16, 32 and 64
-// lanes are taken.  32768 rows of 640, gated, take 25 us on 16 lanes of 5 chunks
-// (64 of 2: 37), 8192 of 1280 15.4 on 32 of 5 (128 of 2: 16.4).  Elsewhere fewer
-// lanes of more chunks lose: 4096 of 2560, normed, 38 on 64 of 5 (192 of 2: 17).
+// lanes are taken.  32768 rows of 640, gated, take 26 us on 16 lanes of 5 chunks
+// (64 of 2: 37), 8192 of 1280 15.4 on 32 of 5 (128 of 2: 16.4), in calls in a row on
+// one input (the former 28 to 30 where inputs change, 27.4 at the least in a trace).
+// Elsewhere fewer lanes of more chunks lose: 4096 of 2560, normed, 38 on 64 of 5
+// (192 of 2: 17).
 template <int KIND, int TX, int TR, int TW>
 static int launch_g128(RowArgs a, hipStream_t st) {
   const int chunks = (a.H + 7) / 8;

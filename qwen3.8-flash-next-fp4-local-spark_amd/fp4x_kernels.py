@@ -249,8 +249,7 @@ def w8a8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
 
 
 # ----------------------------------------------------------------- e4m3 with a scale per block of 128, experts
-# Host side compiled and outputs without gradients, as above; expert_combine_grad and expert_combine are the gradients
-# of sorting tokens by expert and back, for a training loop to call.
+# Host side compiled and outputs without gradients, as above.
 def quantize_f8(w):
     """A weight [N, K], or [E, N, K] for experts, in e4m3 with a scale per 128 x
     128 block: (float8_e4m3fn codes of its shape, fp32 scales [.., ceil(N/128),
@@ -264,16 +263,17 @@ def f8_linear(xq, xs, wq, ws, bias=None, out_dtype=torch.bfloat16):
     + bias[n] over the blocks b of 128 values of K: float8_e4m3fn activations
     [M, K] with fp32 scales [M, ceil(K/128)] (fmt "e4m3_g128" above; of any
     strides, but fastest as that lays them out), weights [N, K] with scales per
-    128 x 128 block (quantize_f8).  Blocks are summed in fp32.  Any M and N, K up
-    to 131071; out_dtype bf16 or fp16, whose products are the matrix cores' fp8
-    ones, or fp32, for which they are exact, at half of the rate.  The fp8 ones are
-    added eight at a time, each cut towards zero to 2^-13 of the largest: 1.5e-5 of
-    a sum of normal values, at worst 8.5e-4 of the largest product of each eight
-    (more than half a step of fp16, and not relative to a result in which larger
-    products cancel; cast an fp32 result where that counts).  Code rows that do not
-    start on 16 bytes are copied first, and rows that do not start on a line of
-    128 take up to a fifth longer (the quantizers lay theirs on lines where that
-    adds little); a bias that is not fp32 is converted in every call."""
+    128 x 128 block (quantize_f8).  Blocks are summed in fp32.  M and N go to 2^24,
+    M N to 2^37, K to 131071; out_dtype bf16 or fp16, whose products are the matrix
+    cores' fp8 ones, or fp32, for which they are exact, at half of the rate.  The
+    fp8 ones are added eight at a time, each cut towards zero to 2^-13 of the
+    largest: 1.5e-5 of a sum of normal values, at worst 8.5e-4 of the largest
+    product of each eight (more than half a step of fp16, and not relative to a
+    result in which larger products cancel; cast an fp32 result where that counts).
+    Code rows that do not start on 16 bytes are copied first, and rows that do not
+    start on a line of 128 take up to a fifth longer (the quantizers lay theirs on
+    lines where that adds little); a bias that is not fp32 is converted in every
+    call."""
     return _L.host().f8_linear(xq, xs, wq, ws, bias, out_dtype)
 
 
@@ -284,7 +284,9 @@ def f8_linear_experts(xq, xs, wq, ws, offsets, tokens=None, out_dtype=torch.bflo
     (the first product after expert_sort; nothing is gathered in memory);
     without, of row s (the second).  offsets is int32 [E + 1], as expert_sort
     gives it; rows from offsets[E] on are not written.  At most 4096 experts;
-    rows that tokens pick from lie within 2^32 bytes."""
+    rows that tokens pick from lie within 2^32 bytes.  The kernel's tiles are chosen
+    for P rows: where many pairs have no expert here and the host knows how many
+    have, tokens (or xq) cut to those rows are up to a third faster."""
     return _L.host().f8_linear_experts(xq, xs, wq, ws, offsets, tokens, out_dtype)
 
 
@@ -300,15 +302,18 @@ def expert_sort(ids, experts):
 
 def expert_rows(x, tokens):
     """x[tokens] [P, H] of rows x [T, H] of any type of 1, 2 or 4 bytes; rows whose
-    token is not in 0 .. T - 1 are zeros.  The gradient of x is
-    expert_combine(the rows' gradient, slots)."""
+    token is not in 0 .. T - 1 are zeros.  The result carries no autograd graph, also
+    where x requires a gradient: that of x is expert_combine(the rows' gradient,
+    slots), for the caller to apply (an autograd.Function's backward)."""
     return _L.host().expert_rows(x, tokens)
 
 
 def expert_combine(y, slots, weights=None):
     """out[t] = sum_j weights[t, j] * y[slots[t, j]] (ones without weights), summed
     in fp32 in the order of j, in y's type.  y [P, H], slots int32 [T, k], weights
-    [T, k] bf16, fp16 or fp32.  Pairs whose slot is not in 0 .. P - 1 are left out."""
+    [T, k] bf16, fp16 or fp32.  Pairs whose slot is not in 0 .. P - 1 are left out.
+    The result carries no autograd graph, also where y or weights require a gradient:
+    those are expert_combine_grad's, for the caller to apply."""
     return _L.host().expert_combine(y, slots, weights)
 
 
